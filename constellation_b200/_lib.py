@@ -23,6 +23,7 @@ CST_ERR_DEVICE_TIMEOUT = 7
 CST_DTYPE_FP16 = 1
 CST_DTYPE_BF16 = 2
 CST_DTYPE_FP32 = 3
+CST_DTYPE_E4M3 = 4
 
 CST_FLAG_ADD_SHARED = 1
 
@@ -36,6 +37,8 @@ EXPORTED = (
     "cst_ipc_alloc", "cst_ipc_open", "cst_ipc_close", "cst_ipc_free", "cst_moe_routed_push", "cst_reduce_pushed",
     "cst_encode_infer_request", "cst_decode_infer_request", "cst_encode_infer_response", "cst_decode_infer_response",
     "cst_serve_infer_request", "cst_gather_rows", "cst_set_expert_own_tokens_only",
+    "cst_add_rmsnorm", "cst_sort_routes", "cst_sort_rows", "cst_unsort_rows", "cst_unsort_rows_grad",
+    "cst_int4_bytes", "cst_int4_pack", "cst_grouped_int4",
 )
 CST_INFER_REQUEST_FIXED_BYTES = 24
 CST_INFER_RESPONSE_FIXED_BYTES = 20
@@ -75,6 +78,11 @@ class CstExpertWeights(ctypes.Structure):
         ("row_block", ctypes.c_int32),
         ("col_block", ctypes.c_int32),
     ]
+
+
+class CstInt4Weight(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("n_experts", "n", "k", "group", "scale_dtype", "has_zero",
+                                                    "swiglu")]
 
 
 class CstError(RuntimeError):
@@ -123,6 +131,15 @@ def _load() -> ctypes.CDLL:
         "cst_set_shared_slot": (ctypes.c_int, [P, I32]),
         "cst_set_gemm_mode": (ctypes.c_int, [P, I32]),
         "cst_rmsnorm": (ctypes.c_int, [P, I32, I32, I32, P, ctypes.c_float, P, I32, P]),
+        "cst_add_rmsnorm": (ctypes.c_int, [P, I32, I64, P, I32, I64, I32, I32, P, F, P, I64, P, I32, I64, P, P]),
+        "cst_sort_routes": (ctypes.c_int, [P, I32, I32, I32, I32, I32, P, P, P, P]),
+        "cst_sort_rows": (ctypes.c_int, [P, I64, I64, P, I32, I64, I32, I32, P, P, P, P, P]),
+        "cst_unsort_rows": (ctypes.c_int, [P, I32, I64, P, P, I32, I32, I32, P, I32, I64, P, I32, P]),
+        "cst_unsort_rows_grad": (ctypes.c_int, [P, I32, I64, P, I32, I64, P, P, P, I32, I32, I32, P, P, P]),
+        "cst_int4_bytes": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), ctypes.POINTER(I64)]),
+        "cst_int4_pack": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), P, P, P, P, P]),
+        "cst_grouped_int4": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), P, P, I32, I64, P, I64, P, I32, P, I32,
+                                            I64, P]),
         "cst_route": (ctypes.c_int, [P, P, I32, I32, P, P, P, I32, P, P, P, P, P]),
         "cst_moe_routed": (ctypes.c_int, [P, P, I32, I32, P, P, I32, U32, P, I32, P]),
         "cst_moe_routed_range": (ctypes.c_int, [P, P, I32, I32, P, P, I32, I32, I32, P, I32, P]),

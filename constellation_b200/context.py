@@ -9,13 +9,14 @@ arithmetic of the path runs in the library's sm_100a kernels.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import CST_DTYPE_BF16, CST_DTYPE_FP16, CST_DTYPE_FP32, check
+from ._lib import CST_DTYPE_BF16, CST_DTYPE_E4M3, CST_DTYPE_FP16, CST_DTYPE_FP32, check
 
 _DT = {torch.float16: CST_DTYPE_FP16, torch.bfloat16: CST_DTYPE_BF16, torch.float32: CST_DTYPE_FP32}
 _DT_INV = {v: k for k, v in _DT.items()}
@@ -89,6 +90,108 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
         check(_lib.lib.cst_rmsnorm(x.data_ptr(), dtype_code(x.dtype), x.shape[0], x.shape[1], _ptr(weight),
                                    ctypes.c_float(eps), out.data_ptr(), dtype_code(out.dtype), _stream(x.device)))
     return out
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """``torch.cuda.device(device)``, without its cost where that device is the current one."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _no_grad(what: str, *tensors) -> None:
+    """Refuse inputs whose gradient an operator without a backward pass would drop silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad() or on detached tensors")
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A 2-D tensor whose rows are dense, and its row stride in elements: the tensor itself where its
+    strides allow that, else a contiguous copy."""
+    T, H = t.shape
+    if T <= 1:
+        return (t if H <= 1 or t.stride(1) == 1 else t.contiguous()), H
+    if (H > 1 and t.stride(1) != 1) or t.stride(0) < H:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _add_rms_norm(what, x, residual, weight, eps, sum_out, out, out_dtype):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda:
+        raise TypeError(f"{what} expects a 2-D CUDA tensor")
+    T, H = x.shape
+    dev = x.device
+    xt = dtype_code(x.dtype)
+    _no_grad(what, x, residual, weight)
+    if weight is not None:
+        if weight.dtype != torch.float32 or weight.shape != (H,) or weight.device != dev:
+            raise RuntimeError("weight must be fp32 [H] on the device of x")
+        weight = weight.contiguous()
+    x, ldx = _rows(x)
+    rt, ldr, lds = 0, 0, 0
+    if residual is not None:
+        rt = dtype_code(residual.dtype)
+        if residual.shape != x.shape or residual.device != dev:
+            raise RuntimeError("residual must have the shape and device of x")
+        given = residual
+        residual, ldr = _rows(residual)
+        if sum_out is None:
+            sum_out = torch.empty((T, H), dtype=given.dtype, device=dev)
+        elif sum_out.dtype != given.dtype or sum_out.shape != x.shape or sum_out.device != dev:
+            raise RuntimeError("sum_out must have the shape, type and device of residual")
+        lds = _out_rows("sum_out", sum_out)
+    elif sum_out is not None:
+        raise RuntimeError("sum_out without a residual")
+    scale = None
+    if out_dtype is None:
+        if out is None:
+            out = torch.empty((T, H), dtype=x.dtype, device=dev)
+        elif out.shape != x.shape or out.device != dev:
+            raise RuntimeError("out must have the shape and device of x")
+        ot = dtype_code(out.dtype)
+        ldo = _out_rows("out", out)
+    else:
+        out = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev)
+        scale = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=dev)
+        ot, ldo = CST_DTYPE_E4M3, H
+    with _on(dev):
+        check(_lib.lib.cst_add_rmsnorm(x.data_ptr(), xt, ldx, _ptr(residual), rt, ldr, T, H, _ptr(weight), eps,
+                                       _ptr(sum_out), lds, out.data_ptr(), ot, ldo, _ptr(scale), _stream(dev)))
+    return out, scale, sum_out
+
+
+def _out_rows(name: str, t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor that is written: its rows have to be dense and apart."""
+    T, H = t.shape
+    if (H > 1 and t.stride(1) != 1) or (T > 1 and t.stride(0) < H):
+        raise RuntimeError(f"{name} must have dense rows that do not overlap")
+    return t.stride(0) if T > 1 else H
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
+                 out: torch.Tensor | None = None, sum_out: torch.Tensor | None = None):
+    """``h = x + residual`` and its RMS norm in one pass (``cst_add_rmsnorm``); returns ``(out, h)``.
+
+    ``out`` is the norm of the unrounded fp32 sum in ``x``'s type (or that of the given ``out``), ``h``
+    the sum in ``residual``'s type.  ``sum_out`` may be ``residual`` (the stream updated in place) or
+    ``x``; ``out`` may be ``x``; other overlaps are not allowed.  Widths up to 32768, any row stride.
+    """
+    if residual is None:
+        raise TypeError("add_rms_norm needs a residual; rms_norm is the norm without one")
+    out, _, h = _add_rms_norm("add_rms_norm", x, residual, weight, eps, sum_out, out, None)
+    return out, h
+
+
+def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                     eps: float = 1e-6, *, sum_out: torch.Tensor | None = None):
+    """``add_rms_norm`` whose result leaves in 8 bits; returns ``(q, scale, h)``.
+
+    ``q`` is e4m3 ``[T, H]``, ``scale`` fp32 ``[T, ceil(H / 128)]``: ``q * scale`` of its 128 columns is the
+    norm, with the block's largest value at 448 (a block of zeros has scale 1).  A NaN stays in its
+    place and does not change its block's scale.  Without ``residual`` the norm is that of ``x`` and
+    ``h`` is None."""
+    return _add_rms_norm("add_rms_norm_fp8", x, residual, weight, eps, sum_out, None, torch.float8_e4m3fn)
 
 
 class ExpertContext:

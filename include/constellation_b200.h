@@ -46,6 +46,7 @@ extern "C" {
 #define CST_DTYPE_FP16 1
 #define CST_DTYPE_BF16 2
 #define CST_DTYPE_FP32 3
+#define CST_DTYPE_E4M3 4 /* only where an entry point says so */
 
 /* cst_moe_layer / cst_moe_routed flags */
 #define CST_FLAG_ADD_SHARED 1u
@@ -247,6 +248,88 @@ int cst_dequant_fp8(const uint8_t* w, const float* scale_inv, int32_t rows, int3
  * NULL (all ones).  x == out is allowed. */
 int cst_rmsnorm(const void* x, int32_t x_dtype, int32_t T, int32_t H, const float* weight, float eps, void* out,
                 int32_t out_dtype, void* stream);
+
+/* Residual add + RMSNorm, optionally leaving in 8 bits, on the current device.  For T rows of
+ * H columns (1 <= H <= 32768):
+ *   h = x + residual (fp32);  sum = h, rounded once to residual_dtype;
+ *   y = h * rsqrt(mean(h^2) + eps) * weight (fp32, from the unrounded h);
+ *   out = y, rounded once -- or, for out_dtype CST_DTYPE_E4M3, with one scale per 128 columns:
+ *   scale[t, b] = max |y| of the block / 448 (1 for a block of zeros), out = e4m3(y / scale).
+ * The prenorm of a sparse layer with the residual before it (server/full_model_runtime.py
+ * :271-276).  residual NULL: none (sum must be NULL too); sum NULL: not kept.  weight [H] fp32
+ * or NULL (ones).  scale [T, ceil(H / 128)] fp32.  ld_*: row strides in elements.  sum may be x
+ * or residual itself and out may be x itself (same address, type and stride); no other overlap. */
+int cst_add_rmsnorm(const void* x, int32_t x_dtype, int64_t ld_x, const void* residual, int32_t residual_dtype,
+                    int64_t ld_residual, int32_t T, int32_t H, const float* weight, float eps, void* sum,
+                    int64_t ld_sum, void* out, int32_t out_dtype, int64_t ld_out, float* scale, void* stream);
+
+/* ---- Tokens sorted by expert and back ---------------------------------------------------
+ * The dispatch and combine of a sparse layer (dispatch_topk_experts and
+ * combine_outputs_torch, server/moe_layer_runtime.py:111-167) around expert products that the
+ * caller runs on rows grouped by expert, on the current device, with their gradients.
+ * A "route" is a (token t, k) pair; T * K <= 2^30, K <= CST_SORT_MAX_TOP_K. */
+#define CST_SORT_MAX_TOP_K 1024
+/* Numbers the routes to experts [first_expert, first_expert + n_experts) (n_experts <= 1024) in
+ * the order (expert, token, k):
+ *   topk_idx [T, K] int32 or int64 (idx_bytes 4 or 8); an id outside the range, negative ones
+ *            among them, is a route to an expert held elsewhere
+ *   row_of   [T, K] int32: the route's row, -1 for a route held elsewhere
+ *   route_of [T * K] int32: t * K + k of each row, -1 behind the last expert's rows
+ *   offsets  [n_experts + 1] int32: first row of each expert; the last entry is the rows in use */
+int cst_sort_routes(const void* topk_idx, int32_t idx_bytes, int32_t T, int32_t K, int32_t n_experts,
+                    int32_t first_expert, int32_t* row_of, int32_t* route_of, int32_t* offsets, void* stream);
+/* rows[row_of[t, k]] = x[t] for rows of row_bytes bytes (any type), and rows_scale[row_of[t, k]] =
+ * scale[t] ([T, n_scale] fp32, or NULL).  rows [T * K, row_bytes] and rows_scale [T * K, n_scale]
+ * are packed; rows from *rows_used (the last of the offsets, device memory) on are set to zero. */
+int cst_sort_rows(const void* x, int64_t row_bytes, int64_t ld_bytes, const float* scale, int32_t n_scale,
+                  int64_t ld_scale, int32_t T, int32_t K, const int32_t* row_of, const int32_t* rows_used,
+                  void* rows, float* rows_scale, void* stream);
+/* out[t] = sum_k weight[t, k] * rows[row_of[t, k]] (+ residual[t]), fp32 sums in the order of k,
+ * one rounding; out [T, H] packed.  weight [T, K] fp32 or NULL (ones: the gradient of
+ * cst_sort_rows).  A route held elsewhere adds nothing, whatever its weight. */
+int cst_unsort_rows(const void* rows, int32_t rows_dtype, int64_t ld_rows, const int32_t* row_of,
+                    const float* weight, int32_t T, int32_t K, int32_t H, const void* residual,
+                    int32_t residual_dtype, int64_t ld_residual, void* out, int32_t out_dtype, void* stream);
+/* The gradients of cst_unsort_rows for grad [T, H]: d_rows[row_of[t, k]] = weight[t, k] * grad[t] in
+ * rows_dtype ([T * K, H] packed, zero from *rows_used on), d_weight[t, k] = <grad[t],
+ * rows[row_of[t, k]]> in fp32 (0 for a route held elsewhere).  Either may be NULL; rows is
+ * read for d_weight only.  row_of has to be an order of cst_sort_routes (no row twice). */
+int cst_unsort_rows_grad(const void* grad, int32_t grad_dtype, int64_t ld_grad, const void* rows, int32_t rows_dtype,
+                         int64_t ld_rows, const int32_t* row_of, const float* weight, const int32_t* rows_used,
+                         int32_t T, int32_t K, int32_t H, void* d_rows, float* d_weight, void* stream);
+
+/* ---- Products with 4-bit weights ----------------------------------------------------------
+ * Experts (or one dense projection, n_experts 1) whose weights are 4-bit integers with one
+ * scale, and optionally one zero point, for `group` consecutive k of a weight row:
+ *   W[e, n, k] = scale[e, n, k / group] * (q[e, n, k] - zero[e, n, k / group]),  zero = 8 if none.
+ * The reference keeps experts in FP8 only (expert_node_v2/expert_format_v2.h:59-86). */
+#define CST_INT4_MAX_EXPERTS 1024
+typedef struct cst_int4_weight {
+    int32_t n_experts;   /* <= CST_INT4_MAX_EXPERTS */
+    int32_t n, k;        /* weight rows and columns, <= 2^20 */
+    int32_t group;       /* 32, 64 or 128; divides k */
+    int32_t scale_dtype; /* CST_DTYPE_FP16, BF16 or FP32 */
+    int32_t has_zero;
+    int32_t swiglu;      /* 1: rows [0, n/2) are "up", [n/2, n) "gate", and a product returns
+                          * silu(gate) * up, n / 2 columns */
+} cst_int4_weight;
+/* Bytes of the kernels' layout of such a weight. */
+int cst_int4_bytes(const cst_int4_weight* w, int64_t* bytes);
+/* Lays the weight out in `data` (cst_int4_bytes bytes, 16-byte aligned, device) from q
+ * [n_experts, n, k / 2] (two values a byte, the lower k in the lower half), scale
+ * [n_experts, n, k / group] in scale_dtype and zero [n_experts, n, k / group] uint8 (0..15; NULL
+ * without zero points).  Load-time, stream-ordered. */
+int cst_int4_pack(const cst_int4_weight* w, const uint8_t* q, const void* scale, const uint8_t* zero, void* data,
+                  void* stream);
+/* out[r] = W[e] x[r] for the rows r in [offsets[e], offsets[e + 1]) of each expert (device int32
+ * [n_experts + 1], ascending; entries are clamped to [0, R]), zero for the rows outside;
+ * offsets NULL: one expert, every row.
+ *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise)
+ *   out  [R, n] (n / 2 with swiglu) in out_dtype (fp16, bf16, fp32)
+ * fp32 sums of exact products, one rounding. */
+int cst_grouped_int4(const cst_int4_weight* w, const void* data, const void* x, int32_t x_dtype, int64_t ld_x,
+                     const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* out,
+                     int32_t out_dtype, int64_t ld_out, void* stream);
 
 /* ---- Peer-memory exchange (expert parallelism, one process per GPU, NVLink) -----------
  * No counterpart in the reference: its coordinator collects one expert result per
