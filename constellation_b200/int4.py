@@ -62,8 +62,7 @@ class Int4Weight:
         if scale.dim() != 3 or scale.shape[:2] != (E, N) or not scale.shape[2] or K % scale.shape[2]:
             raise RuntimeError(f"scale must be [{E}, {N}, {K} / group], got {tuple(scale.shape)}")
         self._init(E, N, K, K // scale.shape[2], scale.dtype, zero is not None, swiglu, q.device)
-        for e in range(E):
-            self.load(e, q[e], scale[e], None if zero is None else zero[e])
+        self._pack(0, E, q, scale, zero)
 
     @classmethod
     def empty(cls, n_experts: int, n: int, k: int, *, group: int = 128, scale_dtype: torch.dtype = torch.float16,
@@ -78,35 +77,41 @@ class Int4Weight:
             raise RuntimeError(f"Int4Weight needs a CUDA device, got {device}")
         self._c = _lib.CstInt4Weight(int(E), int(N), int(K), int(group), dtype_code(scale_dtype), int(has_zero),
                                      int(bool(swiglu)))
-        self._one = _lib.CstInt4Weight(1, *(getattr(self._c, f) for f, _ in self._c._fields_[1:]))
         self._ref = ctypes.byref(self._c)
         size = ctypes.c_int64()
-        check(_lib.lib.cst_int4_bytes(ctypes.byref(self._one), ctypes.byref(size)))
-        check(_lib.lib.cst_int4_bytes(self._ref, ctypes.byref(ctypes.c_int64())))
+        check(_lib.lib.cst_int4_bytes(self._ref, ctypes.byref(size)))
         self.n_experts, self.n, self.k, self.group = int(E), int(N), int(K), int(group)
         self.scale_dtype, self.zero_points, self.swiglu = scale_dtype, bool(has_zero), bool(swiglu)
         self.out_features = self.n // 2 if swiglu else self.n
-        self.data = torch.zeros((self.n_experts, size.value), dtype=torch.uint8, device=device)
+        self.data = torch.zeros(size.value, dtype=torch.uint8, device=device)
         self.device = self.data.device
 
     def load(self, expert: int, q: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None) -> None:
         """Lay expert ``expert``'s ``q [N, K / 2]``, ``scale`` and ``zero`` ``[N, K / group]`` out (stream-ordered)."""
         if not 0 <= expert < self.n_experts:
             raise IndexError(f"expert {expert} outside [0, {self.n_experts})")
+        self._pack(int(expert), 1, q[None], scale[None], None if zero is None else zero[None])
+
+    def _pack(self, first, count, q, scale, zero):
         G = self.k // self.group
         if (zero is not None) != self.zero_points:
             raise RuntimeError("zero points are given for all experts of a weight or for none")
-        for name, t, shape, dtype in (("q", q, (self.n, self.k // 2), torch.uint8),
-                                      ("scale", scale, (self.n, G), self.scale_dtype),
-                                      ("zero", zero, (self.n, G), torch.uint8)):
+        for name, t, shape, dtype in (("q", q, (count, self.n, self.k // 2), torch.uint8),
+                                      ("scale", scale, (count, self.n, G), self.scale_dtype),
+                                      ("zero", zero, (count, self.n, G), torch.uint8)):
             if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device):
-                raise RuntimeError(f"{name} must be {dtype} {shape} on {self.device}, got {t.dtype} "
-                                   f"{tuple(t.shape)} on {t.device}")
+                raise RuntimeError(f"{name} must be {dtype} {list(shape)} on {self.device}, got {t.dtype} "
+                                   f"{list(t.shape)} on {t.device}")
         q, scale = q.contiguous(), scale.contiguous()
         zero = zero.contiguous() if zero is not None else None
         with _on(self.device):
-            check(_lib.lib.cst_int4_pack(ctypes.byref(self._one), q.data_ptr(), scale.data_ptr(), _ptr(zero),
-                                         self.data[expert].data_ptr(), _stream(self.device)))
+            check(_lib.lib.cst_int4_pack(self._ref, first, count, q.data_ptr(), scale.data_ptr(), _ptr(zero),
+                                         self.data.data_ptr(), _stream(self.device)))
+
+    def device_error(self) -> None:
+        """Wait for the current stream and raise if a product's bounded device-side wait gave up."""
+        with _on(self.device):
+            check(_lib.lib.cst_int4_device_error(self._ref, self.data.data_ptr(), _stream(self.device)))
 
 
 def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = None, *,
@@ -155,6 +160,9 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
         raise RuntimeError(f"out must be contiguous [{R}, {w.out_features}] on the device of x")
     ot = dtype_code(out.dtype)
     x, ldx = _rows(x)
+    size = x.element_size()
+    if x.data_ptr() % 16 or ldx * size % 16:  # the kernel copies whole 16-byte pieces of a row
+        x, ldx = x.clone(memory_format=torch.contiguous_format), K
     lds = 0
     if x_scale is not None:
         x_scale, lds = _rows(x_scale)
@@ -294,3 +302,5 @@ class Int4Experts:
     def device_error(self) -> None:
         """Synchronise and raise if a kernel's bounded device-side wait gave up."""
         self._ctx.device_error()
+        for w in (self.up_gate, self.down, *(self._shared or ())):
+            w.device_error()

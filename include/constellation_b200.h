@@ -313,23 +313,28 @@ typedef struct cst_int4_weight {
     int32_t swiglu;      /* 1: rows [0, n/2) are "up", [n/2, n) "gate", and a product returns
                           * silu(gate) * up, n / 2 columns */
 } cst_int4_weight;
-/* Bytes of the kernels' layout of such a weight. */
+/* Bytes of the kernels' layout of such a weight, and of its device error word behind it. */
 int cst_int4_bytes(const cst_int4_weight* w, int64_t* bytes);
-/* Lays the weight out in `data` (cst_int4_bytes bytes, 16-byte aligned, device) from q
- * [n_experts, n, k / 2] (two values a byte, the lower k in the lower half), scale
- * [n_experts, n, k / group] in scale_dtype and zero [n_experts, n, k / group] uint8 (0..15; NULL
- * without zero points).  Load-time, stream-ordered. */
-int cst_int4_pack(const cst_int4_weight* w, const uint8_t* q, const void* scale, const uint8_t* zero, void* data,
-                  void* stream);
+/* Lays the experts [first, first + count) of the weight out in `data` (cst_int4_bytes bytes, zeroed
+ * by the caller before the first call, 16-byte aligned, device) from these experts' q
+ * [count, n, k / 2] (two values a byte, the lower k in the lower half), scale [count, n, k / group] in
+ * scale_dtype and zero [count, n, k / group] uint8 (0..15; NULL without zero points).  An expert that
+ * is not laid out is all zero.  Load-time, stream-ordered. */
+int cst_int4_pack(const cst_int4_weight* w, int32_t first, int32_t count, const uint8_t* q, const void* scale,
+                  const uint8_t* zero, void* data, void* stream);
 /* out[r] = W[e] x[r] for the rows r in [offsets[e], offsets[e + 1]) of each expert (device int32
- * [n_experts + 1], ascending; entries are clamped to [0, R]), zero for the rows outside;
- * offsets NULL: one expert, every row.
- *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise)
+ * [n_experts + 1], ascending; the kernel clamps them to [0, R] and to ascending order), zero for the
+ * rows outside; offsets NULL: one expert, every row.
+ *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise);
+ *        rows 16-byte aligned (base and stride)
  *   out  [R, n] (n / 2 with swiglu) in out_dtype (fp16, bf16, fp32)
- * fp32 sums of exact products, one rounding. */
-int cst_grouped_int4(const cst_int4_weight* w, const void* data, const void* x, int32_t x_dtype, int64_t ld_x,
+ * fp32 sums of exact products, one rounding.  `data` is only read, but for its error word. */
+int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
                      const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* out,
                      int32_t out_dtype, int64_t ld_out, void* stream);
+/* Waits for `stream`, then returns CST_OK or CST_ERR_DEVICE_TIMEOUT if a bounded wait of a product
+ * with this weight gave up since the last call (and clears the word). */
+int cst_int4_device_error(const cst_int4_weight* w, void* data, void* stream);
 
 /* ---- Peer-memory exchange (expert parallelism, one process per GPU, NVLink) -----------
  * No counterpart in the reference: its coordinator collects one expert result per

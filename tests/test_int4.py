@@ -453,21 +453,26 @@ def test_refusals_without_a_device():
         return ctypes.byref(_lib.CstInt4Weight(E, n, k, group, st, z, sw))
 
     size = ctypes.c_int64()
-    assert L.cst_int4_bytes(weight(), ctypes.byref(size)) == 0 and size.value == 4096 + 64 * 2
+    assert L.cst_int4_bytes(weight(), ctypes.byref(size)) == 0 and size.value == 4096 + 64 * 2 + 256
     assert L.cst_int4_bytes(weight(E=3, n=65, k=160, group=32, st=3, z=1), ctypes.byref(size)) == 0
-    assert size.value == 3 * 2 * 2 * (4096 + 4 * 64 * 4 + 4 * 64)
+    assert size.value == 3 * 2 * 2 * (4096 + 4 * 64 * 4 + 4 * 64) + 256
     for kw in (dict(E=0), dict(E=1025), dict(n=0), dict(k=0), dict(group=16), dict(k=130), dict(st=4), dict(n=3, sw=1),
                dict(n=1 << 21)):
         assert L.cst_int4_bytes(weight(**kw), ctypes.byref(size)) == BAD, kw
     assert L.cst_int4_bytes(None, ctypes.byref(size)) == BAD
     for a in ((None, P, None, P), (P, None, None, P), (P, P, None, None), (P, P, None, 8)):
-        assert L.cst_int4_pack(weight(), *a, None) == BAD
-    assert L.cst_int4_pack(weight(z=1), P, P, None, P, None) == BAD
+        assert L.cst_int4_pack(weight(), 0, 1, *a, None) == BAD
+    assert L.cst_int4_pack(weight(z=1), 0, 1, P, P, None, P, None) == BAD
+    for first, count in ((-1, 1), (0, 3), (2, 1), (0, -1)):
+        assert L.cst_int4_pack(weight(E=2), first, count, P, P, None, P, None) == BAD
+    assert L.cst_int4_pack(weight(), 0, 0, None, None, None, None, None) == _lib.CST_OK
+    assert L.cst_int4_device_error(weight(), None, None) == BAD
 
     def call(w=None, data=P, x=P, xt=2, ldx=128, xs=None, lds=1, off=P, R=1, out=P, ot=2, ldo=64):
         return L.cst_grouped_int4(w or weight(), data, x, xt, ldx, xs, lds, off, R, out, ot, ldo, None)
 
     assert call(data=None, x=None, out=None, R=0) == _lib.CST_OK
     for kw in (dict(xt=3), dict(xt=4), dict(xs=P), dict(ot=4), dict(ldx=127), dict(ldo=63), dict(R=-1), dict(x=None),
-               dict(out=None), dict(data=None), dict(w=weight(E=2), off=None), dict(xt=4, xs=P, lds=0)):
+               dict(out=None), dict(data=None), dict(w=weight(E=2), off=None), dict(xt=4, xs=P, lds=0),
+               dict(x=8), dict(ldx=129)):
         assert call(**kw) == BAD, kw
