@@ -356,8 +356,8 @@ __device__ __forceinline__ Item find_item(const Int4Args& a, const int* s_tile, 
     return it;
 }
 
-template <XType X, int GROUPS>
-__global__ void __launch_bounds__(kThreads, 1) int4_kernel(Int4Args a) {
+template <XType X, int GROUPS, bool WIDE>
+__global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) int4_kernel(Int4Args a) {
     extern __shared__ __align__(128) uint8_t s_ring[];
     __shared__ int s_tile[CST_INT4_MAX_EXPERTS + 1], s_row[CST_INT4_MAX_EXPERTS + 1];
     __shared__ int s_scan[kThreads / 32][2];
@@ -552,8 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(Int4Args a) {
                 }
             };
             if (it.rows <= 8) product(std::integral_constant<int, 1>{});
-            else if (it.rows <= 16) product(std::integral_constant<int, 2>{});
-            else product(std::integral_constant<int, 4>{});
+            else if (!WIDE || it.rows <= 16) product(std::integral_constant<int, 2>{});
+            else if constexpr (WIDE) product(std::integral_constant<int, 4>{});
             consumer_sync();
             // the slices' sums, and over a cluster the CTAs', in fixed order
             const int values = it.rows * kRows;
@@ -626,10 +626,10 @@ int choose_ranks(int64_t items, int all_stages, int sms) {
     return best;
 }
 
-template <XType X, int GROUPS>
+template <XType X, int GROUPS, bool WIDE>
 cudaError_t launch_int4(Int4Args a, int sms, cudaStream_t stream) {
-    constexpr int kShared = 216 * 1024;
-    a.tile = choose_tile(a.R, a.g.E);
+    constexpr int kShared = WIDE ? 216 * 1024 : 103 * 1024;
+    sms *= WIDE ? 1 : 2;
     a.x_at = kSlices * a.g.chunk_bytes;
     a.xs_at = a.x_at + a.tile * x_pitch<X>();
     a.stage_bytes = (a.xs_at + (X == XType::e4m3 ? a.tile * kSlices * 4 : 0) + 127) / 128 * 128;
@@ -642,7 +642,7 @@ cudaError_t launch_int4(Int4Args a, int sms, cudaStream_t stream) {
     a.stages = (kShared - sums) / a.stage_bytes;
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     const int64_t clusters = most < sms / a.ranks ? most : sms / a.ranks;
-    auto kernel = int4_kernel<X, GROUPS>;
+    auto kernel = int4_kernel<X, GROUPS, WIDE>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -661,11 +661,17 @@ cudaError_t launch_int4(Int4Args a, int sms, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+template <XType X, int GROUPS>
+cudaError_t launch_tile(Int4Args a, int sms, cudaStream_t s) {
+    a.tile = choose_tile(a.R, a.g.E);
+    return a.tile > 16 ? launch_int4<X, GROUPS, true>(a, sms, s) : launch_int4<X, GROUPS, false>(a, sms, s);
+}
+
 template <XType X>
 cudaError_t launch_groups(const Int4Args& a, int sms, cudaStream_t s) {
-    return a.g.group == 128 ? launch_int4<X, 1>(a, sms, s)
-           : a.g.group == 64 ? launch_int4<X, 2>(a, sms, s)
-                             : launch_int4<X, 4>(a, sms, s);
+    return a.g.group == 128 ? launch_tile<X, 1>(a, sms, s)
+           : a.g.group == 64 ? launch_tile<X, 2>(a, sms, s)
+                             : launch_tile<X, 4>(a, sms, s);
 }
 
 int check_weight(const cst_int4_weight* w) {
