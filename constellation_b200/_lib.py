@@ -39,6 +39,7 @@ EXPORTED = (
     "cst_serve_infer_request", "cst_gather_rows", "cst_set_expert_own_tokens_only",
     "cst_add_rmsnorm", "cst_sort_routes", "cst_sort_rows", "cst_unsort_rows", "cst_unsort_rows_grad",
     "cst_int4_bytes", "cst_int4_pack", "cst_grouped_int4", "cst_int4_device_error",
+    "cst_int4_workspace",
 )
 CST_INFER_REQUEST_FIXED_BYTES = 24
 CST_INFER_RESPONSE_FIXED_BYTES = 20
@@ -138,8 +139,9 @@ def _load() -> ctypes.CDLL:
         "cst_unsort_rows_grad": (ctypes.c_int, [P, I32, I64, P, I32, I64, P, P, P, I32, I32, I32, P, P, P]),
         "cst_int4_bytes": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), ctypes.POINTER(I64)]),
         "cst_int4_pack": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), I32, I32, P, P, P, P, P]),
+        "cst_int4_workspace": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), I32, I32, ctypes.POINTER(I64)]),
         "cst_int4_device_error": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), P, P]),
-        "cst_grouped_int4": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), P, P, I32, I64, P, I64, P, I32, P, I32,
+        "cst_grouped_int4": (ctypes.c_int, [ctypes.POINTER(CstInt4Weight), P, P, I32, I64, P, I64, P, I32, P, P, I32,
                                             I64, P]),
         "cst_route": (ctypes.c_int, [P, P, I32, I32, P, P, P, I32, P, P, P, P, P]),
         "cst_moe_routed": (ctypes.c_int, [P, P, I32, I32, P, P, I32, U32, P, I32, P]),

@@ -4,18 +4,23 @@
 // for the rows r in [offsets[e], offsets[e + 1]) of expert e; rows behind offsets[E] are zero.
 // x in e4m3 carries one fp32 scale for 128 columns of a row.  With `swiglu` the first half of
 // the N weight rows is "up", the second "gate", and y = silu(gate) * up, [R, N / 2].
-// q - zero is exact in 16 bits and so is e4m3 in fp16, so every product is exact and only the
-// fp32 sums and the one final cast round.
 //
-// Layout of one weight (written once by pack_kernel): blocks of 64 weight rows, each a run of
-// chunks of 128 k; a chunk is 4096 bytes of q in the order the matrix instructions take them,
-// then the 64 rows' scales [128 / group][64], then their zero points [128 / group][64].
-// Inside the 4096 bytes: [row tile of 16][half of 64 k][lane][word j of 4]; lane (g, c) holds
-// rows g and g + 8 and the 8 consecutive k from 8 c of both 32s of its half, a word 4 of them:
-// bits 4 i + 16 e .. of a word hold row g + 8 (i & 1), k = 32 (j >> 1) + 8 c + 4 (j & 1) + 2 (i >> 1) + e,
-// and the word is rotated left by 3, which puts them where dequantising wants them.
-// With swiglu a block is 32 "up" rows and the 32 "gate" rows that go with them.
+// A byte q of 0..15 is the e4m3 number q * 2^-9: 0..7 are its subnormals and 8..15 its first normals, in
+// even steps.  So a pair of logic operations turns 8 packed weights into 8 operands of the 8-bit
+// matrix product, and the zero point is one more product of the same x with a constant operand,
+//     2^-9 sum (q - z) x = sum (q 2^-9) x + sum (-z 2^-9) x,
+// into the same accumulator.  x enters as e4m3 terms, x = s (t1 + t2 / 16 + t3 / 256) with a power of two s that
+// fits the largest |x| of the row: two terms for bf16 (8 bits = 4 + 4), three for fp16 (11 bits); what
+// they drop is below 2^-21 (bf16) or 2^-25 (fp16) of that largest |x|.  e4m3 rows enter as they are, with
+// their scales.  The products are exact and the sums fp32, with one rounding at the end.
+//
+// Layout of one weight (written once by pack_kernel): blocks of 128 weight rows, each a run of
+// chunks of 128 k; a chunk is 8192 bytes of q, then the 128 rows' scales [128 / group][128], then
+// their zero points [128 / group][128].  q: [32 k][row][word of 8 k]; byte j of a word holds k = j in its
+// lower and k = 4 + j in its upper half.
+// With swiglu the rows of a block are 64 "up" rows, each followed by the "gate" row that goes with it.
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -29,7 +34,7 @@ namespace cst {
 
 namespace {
 
-constexpr int kRows = 64;    // weight rows of a block
+constexpr int kRows = 128;   // weight rows of a block
 constexpr int kChunk = 128;  // k of a chunk
 constexpr int kQBytes = kRows * kChunk / 2;
 constexpr int kErrBytes = 256;  // behind the experts: the device error word of the products' bounded waits
@@ -64,8 +69,8 @@ __device__ __forceinline__ int source_row(const Geom& g, int b, int r) {
         const int n = b * kRows + r;
         return n < g.N ? n : -1;
     }
-    const int n = b * (kRows / 2) + (r & 31);
-    return n < g.out_n ? n + (r >= 32 ? g.out_n : 0) : -1;
+    const int n = b * (kRows / 2) + (r >> 1);
+    return n < g.out_n ? n + (r & 1 ? g.out_n : 0) : -1;
 }
 
 // One CTA per (chunk, block, expert).  Padding (rows past N, k past K) gets q = 8 and scale 0,
@@ -75,21 +80,19 @@ __global__ void __launch_bounds__(256) pack_kernel(Geom g, const uint8_t* q, con
     const int chunk = blockIdx.x, b = blockIdx.y, e = blockIdx.z;  // e counts from the first expert of the call
     uint8_t* dst = out + e * g.expert_bytes() + (int64_t(b) * g.chunks + chunk) * g.chunk_bytes;
     for (int w = threadIdx.x; w < kQBytes / 4; w += blockDim.x) {
-        const int j = w & 3, lane = (w >> 2) & 31, half = (w >> 7) & 1, tile = w >> 8;
-        uint32_t word = 0;
-        for (int i = 0; i < 4; ++i) {
-            const int n = source_row(g, b, tile * 16 + (lane >> 2) + 8 * (i & 1));
-            for (int el = 0; el < 2; ++el) {
-                const int k = chunk * kChunk + half * 64 + 32 * (j >> 1) + (lane & 3) * 8 + 4 * (j & 1) + 2 * (i >> 1) + el;
-                uint32_t v = 8;
-                if (n >= 0 && k < g.K) {
-                    const uint8_t two = q[((int64_t(e) * g.N + n) * g.K + k) >> 1];
-                    v = (k & 1) ? two >> 4 : two & 15;
-                }
-                word |= v << (4 * i + 16 * el);
+        // source order: the 16 words of a row one after the other
+        const int n = source_row(g, b, w >> 4), k = chunk * kChunk + (w & 15) * 8;
+        uint32_t word = 0x88888888u;
+        if (n >= 0 && k < g.K) {  // k ends on a multiple of 32
+            const uint8_t* src = q + ((int64_t(e) * g.N + n) * g.K + k) / 2;
+            word = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t v = i & 1 ? src[i >> 1] >> 4 : src[i >> 1] & 15;
+                word |= v << (8 * (i & 3) + 4 * (i >> 2));
             }
         }
-        reinterpret_cast<uint32_t*>(dst)[w] = (word << 3) | (word >> 29);
+        reinterpret_cast<uint32_t*>(dst)[(((w & 15) >> 2) * kRows + (w >> 4)) * 4 + (w & 3)] = word;
     }
     for (int s = threadIdx.x; s < kChunk / g.group * kRows; s += blockDim.x) {
         const int n = source_row(g, b, s % kRows), G = chunk * (kChunk / g.group) + s / kRows;
@@ -103,13 +106,140 @@ __global__ void __launch_bounds__(256) pack_kernel(Geom g, const uint8_t* q, con
     }
 }
 
+// ---- the rows of x as e4m3 terms -----------------------------------------------------------
+
+constexpr int kFactBytes = 16;  // of an e4m3 row and chunk: its scale, padded to what a bulk copy takes
+
+// One CTA a row.  terms: [rows * TERMS][chunks * 128], columns past k zero.  facts: the rows' s; for e4m3
+// (TERMS 1) [chunks][rows] of x_scale, 16 bytes each.  A row's first 8192 columns stay in registers between
+// its maximum and its terms; more are read twice.
+template <int TERMS>
+__global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype, int64_t ld, const float* x_scale,
+                                                      int64_t ld_xs, int rows, int k, uint8_t* terms, float* facts) {
+    __shared__ float s_most[8];
+    chain_wait();
+    chain_release();
+    const int chunks = (k + kChunk - 1) / kChunk, width = chunks * kChunk;
+    const int64_t r = blockIdx.x, at = r * ld;
+    if constexpr (TERMS == 1) {
+        const uint8_t* src = static_cast<const uint8_t*>(x) + at;
+        const bool vec = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+        for (int c = threadIdx.x * 16; c < width; c += blockDim.x * 16) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c < k) {  // k is a multiple of 32
+                if (vec) {
+                    v = *reinterpret_cast<const uint4*>(src + c);
+                } else {
+                    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j >> 2] |= uint32_t(src[c + j]) << (8 * (j & 3));
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            *reinterpret_cast<uint4*>(terms + r * width + c) = v;
+        }
+        for (int c = threadIdx.x; c < chunks; c += blockDim.x)
+            facts[(int64_t(c) * rows + r) * (kFactBytes / 4)] = x_scale[r * ld_xs + c];
+        return;
+    }
+    constexpr int kHeld = 4;  // vectors of 8 columns a thread holds
+    const bool vec = (reinterpret_cast<uintptr_t>(x) + at * 2) % 16 == 0;
+    auto load = [&](int c, float (&v)[8]) {
+        if (vec) {
+            load_act<8>(x, x_dtype, at + c, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float e[1];
+                load_act<1>(x, x_dtype, at + c + j, e);
+                v[j] = e[0];
+            }
+        }
+        // e4m3 has no infinities: one makes its row's results NaN, as a NaN does
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (isinf(v[j])) v[j] = __int_as_float(0x7fffffff);
+    };
+    const int step = blockDim.x * 8, first = threadIdx.x * 8;
+    float held[kHeld][8], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int c = first + i * step;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) held[i][j] = 0.0f;
+        if (c < k) load(c, held[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(held[i][j]));
+    }
+    for (int c = first + kHeld * step; c < k; c += step) {
+        float v[8];
+        load(c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+    }
+    most = warp_max_nonneg(most);
+    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) most = fmaxf(most, s_most[w]);
+    const float scale = pow2_scale_for(most), inv = pow2_recip(scale);
+    if (threadIdx.x == 0) facts[r] = scale;
+    auto store = [&](int c, const float (&x8)[8]) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x8[j] * inv;
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                q[j] = e4m3x2_rn(v[2 * j], v[2 * j + 1]);
+                const float2 f = e4m3x2_to_f32x2(q[j]);
+                // exact: the rest has fewer bits than v; its largest is 16, which 16-fold stays below 448
+                v[2 * j] = (v[2 * j] - f.x) * 16.0f;
+                v[2 * j + 1] = (v[2 * j + 1] - f.y) * 16.0f;
+            }
+            *reinterpret_cast<uint2*>(terms + (r * TERMS + t) * width + c) =
+                make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (first + i * step < width) store(first + i * step, held[i]);
+    for (int c = first + kHeld * step; c < width; c += step) {
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (c < k) load(c, v);
+        store(c, v);
+    }
+}
+
+// ---- the product ---------------------------------------------------------------------------
+// One persistent CTA per SM walks items (row tile of an expert, block of 128 weight rows); the
+// CTAs of a cluster split an item's k.  Per step of up to four chunks of 128 k:
+//   warp 0     producer: one bulk copy of the packed weights with their scales (8.4 KB a chunk), TMA tiles of
+//              x's terms [tile * TERMS][128 k], swizzled as the matrix unit reads them (and for e4m3 the
+//              rows' scales), into a ring;
+//   warps 2..  four wideners: each thread owns a weight row, turns its 64 packed bytes into 128 e4m3
+//              numbers with 48 logic operations and stores them to tensor memory, where they are the matrix
+//              product's A operand (and the row's zero points, if there are any);
+//   warp 1     one lane issues the tcgen05 products, a fresh fp32 accumulator for each group;
+//   the last   four output warps: each thread owns a weight row of the accumulators:
+//              acc[t] += 2^9 scale * (D1[t] + D2[t] / 16 + D3[t] / 256), and at the end of an item the results.
+// So each weight byte is read once from HBM and once from shared memory, and never goes back there.
+
+constexpr int kMaxStages = 12;
+constexpr int kMaxStep = 4;                     // chunks of a step, which the roles hand on at a time
+constexpr int kWidenSets = 1, kOutSets = 1;     // sets of 4 warps, which take the chunks of a step in turn
+constexpr int kWarpMma = 1, kWarpWiden = 2, kWarpOut = kWarpWiden + 4 * kWidenSets;
+constexpr int kThreads = (kWarpOut + 4 * kOutSets) * 32;
+constexpr int kMaxBufs = 4;                     // steps in tensor memory
+constexpr int kACols = kChunk / 4;              // columns of A: [128 rows][128 k] of 8 bits
+constexpr int kMostColumns = 512 / 2 - kACols - 32;  // accumulator columns of a chunk with which two steps fit
+
 struct Int4Args {
     Geom g;
     const uint8_t* data;
-    const uint8_t* x;
-    int64_t ld_x;  // bytes
-    const float* x_scale;
-    int64_t ld_xs;
+    const float* facts;      // the rows' scales; e4m3: [chunks][R] of x's, kFactBytes each
     const int32_t* offsets;  // null: every row belongs to expert 0
     int R;
     void* out;
@@ -117,62 +247,15 @@ struct Int4Args {
     int64_t ld_out;
     int* err;
     int tile;         // rows of x of an item: 8, 16 or 32
-    int ranks;        // CTAs of a cluster, which split k
+    int ranks;        // CTAs of a cluster
     int stages;       // ring depth
-    int stage_bytes;  // weights, then x, then x scales
-    int x_at, xs_at;  // offsets in a stage
+    int stage_bytes;  // x [step][tile * TERMS][128], then the chunks, then for e4m3 the facts [step][tile]
+    int q_at, f_at;   // offsets in a stage
+    int step;         // chunks of a step
+    int bufs;         // steps in tensor memory: A, behind all of them the zero points, then the accumulators
+    int z_at, d_at;   // first columns of the zero points (8 for each group of a step, or 8 in all) and accumulators
+    int d_cols;       // columns of one accumulator: tile * TERMS up to a multiple of 16
 };
-
-constexpr int kSlices = 4;                       // chunks of a stage = k slices of the consumer warps
-constexpr int kRowTiles = 2;                     // tiles of 16 weight rows of a warp
-constexpr int kConsumers = kSlices * 4 / kRowTiles;
-constexpr int kThreads = (kConsumers + 1) * 32;  // and the producer warp
-constexpr int kMaxStages = 12;
-
-enum class XType { bf16, f16, e4m3 };
-
-// Bytes of one row of x in a stage.  8 lanes of a 16-byte (16-bit x) or 16 of an 8-byte (e4m3)
-// shared-memory read take 64 (32) bytes of a row each: rows 64 (32) bytes apart mod 128 keep
-// them on different banks.
-template <XType X>
-__host__ __device__ constexpr int x_pitch() {
-    return X == XType::e4m3 ? kSlices * kChunk + 32 : kSlices * kChunk * 2 + 64;
-}
-
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-template <XType X>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (X == XType::bf16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Eight k of x for two matrix instructions: words 0, 1 go with the first, 2, 3 with the second.
-template <XType X>
-__device__ __forceinline__ void load_x(const uint8_t* p, uint32_t (&v)[4]) {
-    if constexpr (X == XType::e4m3) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        const uint32_t w[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i]), __NV_E4M3);
-            v[i] = uint32_t(h.x) | (uint32_t(h.y) << 16);
-        }
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-    }
-}
 
 __device__ __forceinline__ float scale_at(const uint8_t* scales, int dtype, int s) {
     if (dtype == 3) return reinterpret_cast<const float*>(scales)[s];
@@ -180,110 +263,59 @@ __device__ __forceinline__ float scale_at(const uint8_t* scales, int dtype, int 
     return __half2float(reinterpret_cast<const __half*>(scales)[s]);
 }
 
-// The 8 weights of a word as 16 + q in the product's type, exactly: q goes to the top four bits of
-// the mantissa of 2^4, bits 3..6 for bf16 and 6..9 for fp16.
-template <XType X>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t (&a)[4]) {
-    if constexpr (X == XType::bf16) {
-        a[0] = lop_and_or(w, 0x00780078u, 0x41804180u);
-        a[1] = lop_and_or(w >> 4, 0x00780078u, 0x41804180u);
-        a[2] = lop_and_or(w >> 8, 0x00780078u, 0x41804180u);
-        a[3] = lop_and_or(__funnelshift_r(w, w, 12), 0x00780078u, 0x41804180u);
-    } else {
-        a[0] = lop_and_or(w << 3, 0x03c003c0u, 0x4c004c00u);
-        a[1] = lop_and_or(w >> 1, 0x03c003c0u, 0x4c004c00u);
-        a[2] = lop_and_or(w >> 5, 0x03c003c0u, 0x4c004c00u);
-        a[3] = lop_and_or(__funnelshift_r(w, w, 9), 0x03c003c0u, 0x4c004c00u);
-    }
+__device__ __forceinline__ void tma_tile_g2s(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
 }
 
-// One warp: kRowTiles tiles of 16 weight rows times one chunk of k for NT tiles of 8 rows of x.
-// GROUPS: scales of a weight row in the chunk.  sum (q - z) x = sum (16 + q) x - (16 + z) sum x: the
-// second sum comes from a matrix instruction with ones, one for all row tiles, so a weight costs
-// one shift and one logic operation a pair and no subtraction.
-template <XType X, int GROUPS, int NT>
-__device__ __forceinline__ void chunk_product(const Geom& g, const uint8_t* chunk, const uint8_t* x, const float* xs,
-                                              int row_tile, int lane, float (&acc)[kRowTiles][NT][4]) {
-    const int gid = lane >> 2, c = lane & 3, n = row_tile * 16 + gid;
-    constexpr int kX = X == XType::e4m3 ? 1 : 2;
-    constexpr uint32_t kOne = X == XType::bf16 ? 0x3f803f80u : 0x3c003c00u;
-    const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-    float part[kRowTiles][NT][4], sum[NT][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint4 q4[kRowTiles];
-#pragma unroll
-        for (int r = 0; r < kRowTiles; ++r)
-            q4[r] = *reinterpret_cast<const uint4*>(chunk + (((row_tile + r) * 2 + half) * 32 + lane) * 16);
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {  // 32 k
-            const int piece = half * 2 + jj;
-            if (piece % (4 / GROUPS) == 0) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sum[t][i] = 0.0f;
-#pragma unroll
-                        for (int r = 0; r < kRowTiles; ++r) part[r][t][i] = 0.0f;
-                    }
-                }
-            }
-            uint32_t b[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                load_x<X>(x + (t * 8 + gid) * x_pitch<X>() + (piece * 32 + c * 8) * kX, b[t]);
-                mma<X>(sum[t], ones, b[t][0], b[t][1]);
-                mma<X>(sum[t], ones, b[t][2], b[t][3]);
-            }
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-                uint32_t a[4];
-                widen<X>(jj ? q4[r].z : q4[r].x, a);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) mma<X>(part[r][t], a, b[t][0], b[t][1]);
-                widen<X>(jj ? q4[r].w : q4[r].y, a);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) mma<X>(part[r][t], a, b[t][2], b[t][3]);
-            }
-            if (piece % (4 / GROUPS) == 4 / GROUPS - 1) {
-                float s0[NT], s1[NT];
-                if constexpr (X == XType::e4m3) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        s0[t] = xs[(t * 8 + c * 2) * kSlices];
-                        s1[t] = xs[(t * 8 + c * 2 + 1) * kSlices];
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < kRowTiles; ++r) {
-                    const int s = piece / (4 / GROUPS) * kRows + n + r * 16;
-                    const float lo = scale_at(chunk + kQBytes, g.scale_dtype, s);
-                    const float hi = scale_at(chunk + kQBytes, g.scale_dtype, s + 8);
-                    float zlo = -24.0f, zhi = -24.0f;
-                    if (g.has_zero) {
-                        zlo = -16.0f - float(chunk[g.zero_at + s]);
-                        zhi = -16.0f - float(chunk[g.zero_at + s + 8]);
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float p[4] = {fmaf(zlo, sum[t][0], part[r][t][0]), fmaf(zlo, sum[t][1], part[r][t][1]),
-                                      fmaf(zhi, sum[t][2], part[r][t][2]), fmaf(zhi, sum[t][3], part[r][t][3])};
-                        if constexpr (X == XType::e4m3) {
-                            p[0] *= s0[t];
-                            p[1] *= s1[t];
-                            p[2] *= s0[t];
-                            p[3] *= s1[t];
-                        }
-                        acc[r][t][0] = fmaf(p[0], lo, acc[r][t][0]);
-                        acc[r][t][1] = fmaf(p[1], lo, acc[r][t][1]);
-                        acc[r][t][2] = fmaf(p[2], hi, acc[r][t][2]);
-                        acc[r][t][3] = fmaf(p[3], hi, acc[r][t][3]);
-                    }
-                }
-            }
-        }
-    }
+// 32 consecutive 32-bit columns of this thread's lane of tensor memory.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_fill8(uint32_t taddr, uint32_t v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};\n" ::"r"(taddr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+
+// D[tmem] (+)= A[tmem] x B[smem desc], e4m3 x e4m3 -> fp32, K = 32.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(p));
+    return p != 0;
 }
 
 // Arrives on the barrier at the same place of CTA `rank` of the cluster; releases this CTA's
@@ -332,7 +364,33 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
     return false;
 }
 
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory"); }
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+// The clock that bounds a wait costs some hundred cycles to read, so it is left to waits that take long.
+__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, int* err) {
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, err);
+}
+
+// A wait of a whole warp, with one outcome for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
+    return __all_sync(0xffffffffu, lane_wait(bar, parity, err));
+}
+
+// A place in a ring of `n` buffers and the parity of its current pass.
+struct Ring {
+    int i = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++i == n) {
+            i = 0;
+            phase ^= 1;
+        }
+    }
+};
 
 struct Item {
     int expert, row, rows, block;
@@ -356,268 +414,452 @@ __device__ __forceinline__ Item find_item(const Int4Args& a, const int* s_tile, 
     return it;
 }
 
-template <XType X, int GROUPS, bool WIDE>
-__global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) int4_kernel(Int4Args a) {
-    extern __shared__ __align__(128) uint8_t s_ring[];
-    __shared__ int s_tile[CST_INT4_MAX_EXPERTS + 1], s_row[CST_INT4_MAX_EXPERTS + 1];
-    __shared__ int s_scan[kThreads / 32][2];
-    __shared__ uint64_t s_full[kMaxStages], s_empty[kMaxStages], s_join[2];
-    // behind the ring: the k slices' sums of an item, [slice][row of x][weight row], and for a cluster
-    // this CTA's sums of the item and of the one before
-    const int values_cap = a.tile * kRows;
-    float* s_slice = reinterpret_cast<float*>(s_ring + a.stages * a.stage_bytes);
-    float* s_part = s_slice + kSlices * values_cap;
+// First rows (clamped to [0, R], made ascending) and first tiles of the experts, by all threads.
+__device__ __forceinline__ void scan_offsets(const Int4Args& a, int* s_tile, int* s_row, int (*s_scan)[2]) {
+    constexpr int kPer = (CST_INT4_MAX_EXPERTS + kThreads) / kThreads;  // experts + 1 over the threads
+    static_assert(kPer * kThreads >= CST_INT4_MAX_EXPERTS + 1, "every expert needs a thread");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = a.g.E;
+    int row[kPer], most = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = int(threadIdx.x) * kPer + i;
+        int r = 0;
+        if (e <= E) r = a.offsets ? max(0, min(a.offsets[e], a.R)) : (e == 0 ? 0 : a.R);
+        most = max(most, r);
+        row[i] = most;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, most, o);
+        if (lane >= o) most = max(most, v);
+    }
+    if (lane == 31) s_scan[warp][0] = most;
+    int before = __shfl_up_sync(0xffffffffu, most, 1);
+    if (lane == 0) before = 0;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before = max(before, s_scan[w][0]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = int(threadIdx.x) * kPer + i;
+        if (e <= E) s_row[e] = max(row[i], before);
+    }
+    __syncthreads();
+    int tiles[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = int(threadIdx.x) * kPer + i;
+        tiles[i] = sum;
+        if (e < E) sum += (s_row[e + 1] - s_row[e] + a.tile - 1) / a.tile;
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) s_scan[warp][1] = inc;
+    __syncthreads();
+    int base = inc - sum;
+    for (int w = 0; w < warp; ++w) base += s_scan[w][1];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = int(threadIdx.x) * kPer + i;
+        if (e <= E) s_tile[e] = base + tiles[i];
+    }
+    __syncthreads();
+}
+
+// The ring of stages; declared here so that the roles address it as shared memory.
+extern __shared__ __align__(1024) uint8_t s_ring[];
+
+struct Shared {
+    int tile[CST_INT4_MAX_EXPERTS + 1], row[CST_INT4_MAX_EXPERTS + 1];
+    int scan[kThreads / 32][2];
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    // of a buffer in tensor memory: A written and the last accumulators taken; the products done
+    uint64_t ready[kMaxBufs], done[kMaxBufs];
+    uint64_t join[2];
+    uint32_t tmem;
+};
+
+// The work of one CTA: its items, and its steps of k in each.
+struct Span {
+    int64_t items, first, step;
+    int step0, step1;
+};
+
+template <int GROUPS>
+__device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const Span& sp) {
+    const int warp = (int(threadIdx.x) >> 5) - kWarpWiden, lane = threadIdx.x & 31, set = warp >> 2;
+    const int quarter = (int(threadIdx.x) >> 5) & 3;  // the lanes of tensor memory this warp may touch
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    if (!a.g.has_zero) {  // -8 * 2^-9 for every product of this launch; the first arrival below orders it
+        if (set == 0) tmem_fill8(lanes + a.z_at, 0x88888888u);
+    }
+    Ring s, b;
+    for (int64_t i = sp.first; i < sp.items; i += sp.step) {
+        for (int c = sp.step0; c < sp.step1; ++c) {
+            if (!warp_wait(&sh.full[s.i], s.phase, a.err) || !warp_wait(&sh.done[b.i], b.phase ^ 1, a.err)) return;
+            tc_fence_after();
+            const uint8_t* chunk = s_ring + s.i * a.stage_bytes + a.q_at + set * a.g.chunk_bytes + row * 16;
+            uint32_t dst = lanes + (b.i * a.step + set) * kACols;
+            const int n = min(a.step, a.g.chunks - c * a.step);
+#pragma unroll 1
+            for (int h = set; h < n; h += kWidenSets, chunk += kWidenSets * a.g.chunk_bytes, dst += kWidenSets * kACols) {
+                uint32_t v[32];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {  // 32 k
+                    const uint4 q = *reinterpret_cast<const uint4*>(chunk + p * (kRows * 16));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[p * 8 + j * 2] = w[j] & 0x0f0f0f0fu;
+                        v[p * 8 + j * 2 + 1] = (w[j] >> 4) & 0x0f0f0f0fu;
+                    }
+                }
+                tmem_st32(dst, v);
+                if (a.g.has_zero) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) {
+                        const uint32_t z = chunk[a.g.zero_at + g * kRows - row * 15];  // of this row
+                        tmem_fill8(lanes + a.z_at + ((b.i * a.step + h) * GROUPS + g) * 8, (z | 0x80u) * 0x01010101u);
+                    }
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh.ready[b.i]);
+                mbar_arrive(&sh.empty[s.i]);
+            }
+            s.next(a.stages);
+            b.next(a.bufs);
+        }
+    }
+}
+
+// One elected lane.  The operands of an instruction come from uniform registers: under an elected
+// lane, with addresses that are sums of a base and constants, a 128 x 16 x 16 product takes 11 cycles to issue;
+// through a lane that the compiler does not know to be alone it took 160.
+template <int TERMS, int GROUPS>
+__device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Span& sp) {
+    Ring s, b;
+    int used = 0;
+    const uint64_t x0 = umma_desc_sw128(smem_u32(s_ring));
+    const uint32_t x_step = uint32_t(a.stage_bytes) >> 4, x_chunk = uint32_t(a.tile * TERMS) * 8;  // in 16 bytes
+    const uint32_t d_step = uint32_t(a.step * GROUPS * a.d_cols), z_group = a.g.has_zero ? 8 : 0;
+    for (int64_t i = sp.first; i < sp.items; i += sp.step) {
+        const Item it = find_item(a, sh.tile, sh.row, i);
+        const uint32_t idesc = umma_idesc_e4m3(128, (it.rows * TERMS + 15) / 16 * 16);
+        for (int c = sp.step0; c < sp.step1; ++c) {
+            // A is written, and so the stage with its x is full; the accumulators are free
+            if (!lane_wait(&sh.ready[b.i], b.phase, a.err)) goto out;
+            tc_fence_after();
+            const uint64_t x = x0 + uint64_t(uint32_t(s.i) * x_step);
+            const uint32_t w = uint32_t(b.i) * (a.step * kACols), d = uint32_t(a.d_at) + uint32_t(b.i) * d_step;
+            const uint32_t z = uint32_t(a.z_at) + uint32_t(b.i * a.step * GROUPS) * z_group;
+            const int n = min(a.step, a.g.chunks - c * a.step);
+#pragma unroll
+            for (int h = 0; h < kMaxStep; ++h) {
+                if (h >= n) break;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {  // 32 k
+                    const int g = h * GROUPS + ks / (4 / GROUPS);
+                    const uint64_t xk = x + uint32_t(h) * x_chunk + ks * 2;
+                    tc_mma_ts(d + uint32_t(g) * a.d_cols, w + h * kACols + ks * 8, xk, idesc, ks % (4 / GROUPS) > 0);
+                    tc_mma_ts(d + uint32_t(g) * a.d_cols, z + uint32_t(g) * z_group, xk, idesc, true);
+                }
+            }
+            tc_commit(&sh.done[b.i]);
+            used = max(used, b.i + 1);
+            s.next(a.stages);
+            b.next(a.bufs);
+        }
+    }
+out:
+    // tensor memory and the ring stay until the last products are done
+    for (int j = 0; j < used; ++j) lane_wait(&sh.done[j], j < b.i ? b.phase : b.phase ^ 1, a.err);
+}
+
+// N (a multiple of 8) columns from `d` of this thread's lane of tensor memory.
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t d, uint32_t (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j + 16 <= N; j += 16) tmem_ld16(d + j, v + j);
+    if constexpr (N % 16) tmem_ld8(d + N - 8, v + N - 8);
+}
+
+// One item: the sums of ROWS rows of x over the chunks of this set of output warps, for this thread's weight
+// row.
+template <int TERMS, int GROUPS, int ROWS>
+__device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, int set, int row,
+                                           uint32_t lanes, Ring& s, Ring& b, float (&acc)[ROWS]) {
+    constexpr int kAt = ROWS * TERMS <= 32 ? ROWS : 32 / TERMS / 8 * 8;  // rows whose columns are in registers at a time
+    constexpr int kGo = kOutSets == 1 && kAt == ROWS ? 32 / (kAt * TERMS) : 1;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) acc[t] = 0.0f;
+    for (int c = sp.step0; c < sp.step1; ++c) {
+        if (!warp_wait(&sh.done[b.i], b.phase, a.err)) return false;
+        tc_fence_after();
+        const uint8_t* stage = s_ring + s.i * a.stage_bytes;
+        const int n = min(a.step, a.g.chunks - c * a.step) * GROUPS;  // accumulators of the step
+        uint32_t d = a.d_at + lanes + (b.i * a.step + set) * GROUPS * a.d_cols;
+        // (chunk, group) pieces, kGo of them at a time while their columns fit in registers
+#pragma unroll 1
+        for (int p = set * GROUPS; p < n;) {
+            uint32_t v[kGo][kAt * TERMS];
+            float scale[kGo];
+#pragma unroll
+            for (int k = 0; k < kGo; ++k)
+                if (k == 0 || p + k < n) load_columns<kAt * TERMS>(d + k * a.d_cols, v[k]);
+#pragma unroll
+            for (int k = 0; k < kGo; ++k) {
+                const int q = min(p + k, n - 1);
+                scale[k] = scale_at(stage + a.q_at + q / GROUPS * a.g.chunk_bytes + kQBytes, a.g.scale_dtype,
+                                    q % GROUPS * kRows + row) * 512.0f;
+            }
+#pragma unroll
+            for (int t0 = 0; t0 < ROWS; t0 += kAt) {
+                if (t0 > 0) load_columns<kAt * TERMS>(d + t0 * TERMS, v[0]);  // then kGo is 1
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < kGo; ++k) tmem_reg_fence(v[k]);
+#pragma unroll
+                for (int k = 0; k < kGo; ++k) {
+                    if (k > 0 && p + k >= n) break;
+#pragma unroll
+                    for (int t = 0; t < kAt; ++t) {
+                        float y = __uint_as_float(v[k][t * TERMS + TERMS - 1]);
+#pragma unroll
+                        for (int j = TERMS - 2; j >= 0; --j) y = fmaf(y, 0.0625f, __uint_as_float(v[k][t * TERMS + j]));
+                        if constexpr (TERMS == 1)
+                            y *= *reinterpret_cast<const float*>(stage + a.f_at + ((p + k) / GROUPS * a.tile + t0 + t) * kFactBytes);
+                        acc[t0 + t] = fmaf(y, scale[k], acc[t0 + t]);
+                    }
+                }
+            }
+            // on to the next piece, or over the other sets' chunks
+            const int go = kOutSets == 1 ? kGo : p % GROUPS == GROUPS - 1 ? (kOutSets - 1) * GROUPS + 1 : 1;
+            p += go;
+            d += go * a.d_cols;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&sh.ready[b.i]);
+            mbar_arrive(&sh.empty[s.i]);
+        }
+        s.next(a.stages);
+        b.next(a.bufs);
+    }
+    return true;
+}
+
+// Result of weight row `row` of the block for row t of the tile: with swiglu even rows are "up" and
+// their odd neighbours the "gate" that goes with them.
+__device__ __forceinline__ void write_out(const Int4Args& a, const Item& it, int row, int t, float y) {
+    int col = it.block * kRows + row;
+    if (a.g.swiglu) {
+        const float gate = __shfl_down_sync(0xffffffffu, y, 1);
+        y *= gate / (1.0f + expf(-gate));
+        col >>= 1;
+    }
+    const float v[1] = {y};
+    if (col < a.g.out_n && !(a.g.swiglu && (row & 1)))
+        store_act<1>(a.out, a.out_dtype, int64_t(it.row + t) * a.ld_out + col, v);
+}
+
+__device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kOutSets * 128) : "memory"); }
+
+template <int TERMS, int GROUPS>
+__device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s_part, const Span& sp, int rank) {
+    const int lane = threadIdx.x & 31, quarter = (int(threadIdx.x) >> 5) & 3, row = quarter * 32 + lane;
+    const int set = ((int(threadIdx.x) >> 5) - kWarpOut) >> 2, size = a.tile * kRows;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    Ring s, b;
+    bool alive = true;
+    uint32_t turn = 0;
+    if (lane == 0)  // no accumulators to take before the first products
+        for (int j = 0; j < a.bufs; ++j) mbar_arrive(&sh.ready[j]);
+    for (int64_t i = sp.first; i < sp.items; i += sp.step, ++turn) {
+        const Item it = find_item(a, sh.tile, sh.row, i);
+        float* part = s_part + (a.ranks > 1 ? (turn & 1) * kOutSets * size : 0);  // [set][row of x][weight row]
+        auto item = [&](auto rows) {
+            constexpr int ROWS = decltype(rows)::value;
+            float acc[ROWS];
+            alive = alive && accumulate<TERMS, GROUPS, ROWS>(a, sh, sp, set, row, lanes, s, b, acc);
+#pragma unroll
+            for (int t = 0; t < ROWS; ++t) part[set * size + t * kRows + row] = acc[t];
+        };
+        if (it.rows <= 8) item(std::integral_constant<int, 8>{});
+        else if (it.rows <= 16) item(std::integral_constant<int, 16>{});
+        else item(std::integral_constant<int, 32>{});
+        // Lane t has the scale of row t.  (The products above have read x's terms, so it is written.)
+        const float scale = TERMS > 1 && lane < it.rows ? __ldcg(a.facts + it.row + lane) : 1.0f;
+        int t0 = 0, t1 = it.rows;
+        if (a.ranks > 1 || kOutSets > 1) output_sync();
+        if (a.ranks > 1) {
+            // the CTAs' sums over the cluster, in order; two barriers in turn, so that a fast CTA's arrival
+            // for the next item cannot count for this one
+            const int me = int(threadIdx.x) - kWarpOut * 32;
+            if (me < a.ranks) arrive_remote(&sh.join[turn & 1], me);
+            alive = alive && __all_sync(0xffffffffu, wait_cluster(&sh.join[turn & 1], (turn >> 1) & 1, a.err));
+            const int share = (it.rows + a.ranks - 1) / a.ranks;  // rows of x that this CTA writes
+            t0 = rank * share;
+            t1 = min(t0 + share, it.rows);
+        }
+#pragma unroll 4
+        for (int t = t0 + set; t < t1; t += kOutSets) {
+            float y = 0.0f;
+            if (a.ranks == 1) {
+#pragma unroll
+                for (int h = 0; h < kOutSets; ++h) y += part[h * size + t * kRows + row];
+            } else {
+                for (int r = 0; r < a.ranks; ++r)
+#pragma unroll
+                    for (int h = 0; h < kOutSets; ++h) y += load_remote(part + h * size + t * kRows + row, r);
+            }
+            if constexpr (TERMS > 1) y *= __shfl_sync(0xffffffffu, scale, t);
+            write_out(a, it, row, t, y);
+        }
+        // the sums are read before the next item's are written
+        if (a.ranks == 1 && kOutSets > 1) output_sync();
+    }
+}
+
+template <int TERMS, int GROUPS>
+__global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Int4Args a) {
+    __shared__ Shared sh;
+    // behind the ring: the output sets' sums [row of x][weight row] of an item, for a cluster also of the one
+    // before
+    float* s_part = reinterpret_cast<float*>(s_ring + a.stages * a.stage_bytes);
     const Geom& g = a.g;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     const int rank = a.ranks > 1 ? int(blockIdx.x) % a.ranks : 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            // the producer's arrival with the bytes to come; e4m3: its lanes' copies of row scales too
-            mbar_init(&s_full[s], X == XType::e4m3 ? 33 : 1);
-            mbar_init(&s_empty[s], kConsumers);
+            mbar_init(&sh.full[s], 1);  // the producer's arrival with the bytes to come
+            mbar_init(&sh.empty[s], 4 * (kWidenSets + kOutSets));  // the output warps arrive after the products
         }
-        mbar_init(&s_join[0], a.ranks);
-        mbar_init(&s_join[1], a.ranks);
+        for (int b = 0; b < a.bufs; ++b) {
+            mbar_init(&sh.ready[b], 4 * (kWidenSets + kOutSets));
+            mbar_init(&sh.done[b], 1);
+        }
+        mbar_init(&sh.join[0], a.ranks);
+        mbar_init(&sh.join[1], a.ranks);
         fence_barrier_init();
     }
-    if (a.ranks > 1) {  // every CTA's barriers exist before any CTA arrives on them
-        asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
-    } else {
-        __syncthreads();
+    if (warp == kWarpMma) {
+        tmem_alloc(&sh.tmem, 512);  // all of it, so addresses start at column 0
+        tmem_relinquish();
     }
-    chain_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (a.ranks > 1) cluster_barrier();  // every CTA's barriers exist before any CTA arrives on them
+    // The kernel before this one on the stream is split_x_kernel, which let this one start only after it had
+    // waited for everything before it: offsets and weights are there, and `out` is free.  What it writes
+    // itself, x's terms and facts, only the producer reads, after its own wait.
     chain_release();
+    scan_offsets(a, sh.tile, sh.row, sh.scan);
 
-    // first rows (clamped, made ascending) and first tiles of the experts
-    {
-        constexpr int kPer = (CST_INT4_MAX_EXPERTS + kThreads) / kThreads;  // experts + 1 over the threads
-        int row[kPer], carry = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = int(threadIdx.x) * kPer + i;
-            int r = 0;
-            if (e <= g.E) r = a.offsets ? max(0, min(a.offsets[e], a.R)) : (e == 0 ? 0 : a.R);
-            carry = max(carry, r);
-            row[i] = carry;
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, carry, o);
-            if (lane >= o) carry = max(carry, v);
-        }
-        if (lane == 31) s_scan[warp][0] = carry;
-        int before = __shfl_up_sync(0xffffffffu, carry, 1);
-        if (lane == 0) before = 0;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) before = max(before, s_scan[w][0]);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = int(threadIdx.x) * kPer + i;
-            if (e <= g.E) s_row[e] = max(row[i], before);
-        }
-        __syncthreads();
-        int tiles[kPer], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = int(threadIdx.x) * kPer + i;
-            tiles[i] = sum;
-            if (e < g.E) sum += (s_row[e + 1] - s_row[e] + a.tile - 1) / a.tile;
-        }
-        int inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        if (lane == 31) s_scan[warp][1] = inc;
-        __syncthreads();
-        int base = inc - sum;
-        for (int w = 0; w < warp; ++w) base += s_scan[w][1];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = int(threadIdx.x) * kPer + i;
-            if (e <= g.E) s_tile[e] = base + tiles[i];
-        }
-        __syncthreads();
-    }
-    const int64_t items = int64_t(s_tile[g.E]) * g.blocks;
-    const int64_t first = blockIdx.x / a.ranks, step = gridDim.x / a.ranks;
-    // this CTA's chunks of k, whole stages
-    const int all_stages = (g.chunks + kSlices - 1) / kSlices;
-    const int per = (all_stages + a.ranks - 1) / a.ranks;
-    const int chunk0 = min(rank * per * kSlices, g.chunks), chunk1 = min(chunk0 + per * kSlices, g.chunks);
-    constexpr int kX = X == XType::e4m3 ? 1 : 2;
+    Span sp;
+    sp.items = int64_t(sh.tile[g.E]) * g.blocks;
+    sp.first = blockIdx.x / a.ranks;
+    sp.step = gridDim.x / a.ranks;
+    const int steps = (g.chunks + a.step - 1) / a.step, per = (steps + a.ranks - 1) / a.ranks;
+    sp.step0 = min(rank * per, steps);
+    sp.step1 = min(sp.step0 + per, steps);
 
-    if (warp == kConsumers) {
-        int s = 0, issued = 0;
-        uint32_t phase = 0;
-        bool alive = true;
-        for (int64_t i = first; alive && i < items; i += step) {
-            const Item it = find_item(a, s_tile, s_row, i);
+    if (warp == 0) {
+        Ring s;
+        int issued = 0;
+        bool alive = true, waiting = true;
+        for (int64_t i = sp.first; alive && i < sp.items; i += sp.step) {
+            const Item it = find_item(a, sh.tile, sh.row, i);
             const uint8_t* w = a.data + it.expert * g.expert_bytes() + int64_t(it.block) * g.chunks * g.chunk_bytes;
-            const uint8_t* x = a.x + int64_t(it.row + min(lane, it.rows - 1)) * a.ld_x;
-            for (int c = chunk0; c < chunk1; c += kSlices) {
-                alive = mbar_wait(&s_empty[s], phase ^ 1, a.err);
+            for (int c = sp.step0; c < sp.step1; ++c) {
+                alive = warp_wait(&sh.empty[s.i], s.phase ^ 1, a.err);
                 if (!alive) break;
-                uint8_t* stage = s_ring + s * a.stage_bytes;
-                const int n = min(kSlices, chunk1 - c);
-                const int want = n * kChunk, have = min(want, g.K - c * kChunk);  // columns of x
-                uint8_t* xs = stage + a.x_at + lane * x_pitch<X>();
-                if (have < want && lane < it.rows) {
-                    // past k x belongs to someone else: zeros, ordered before this and later bulk copies
-                    for (int b = have * kX; b < want * kX; b += 16)
-                        *reinterpret_cast<uint4*>(xs + b) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
+                uint8_t* stage = s_ring + s.i * a.stage_bytes;
+                const int n = min(a.step, g.chunks - c * a.step);
+                if (elect_one()) {
+                    // a TMA tile always counts whole: what lies past the rows arrives as zeros
+                    mbar_arrive_expect_tx(&sh.full[s.i],
+                                          n * (g.chunk_bytes + a.tile * TERMS * kChunk + (TERMS == 1 ? it.rows * kFactBytes : 0)));
+                    tma_bulk_g2s(stage + a.q_at, w + int64_t(c) * a.step * g.chunk_bytes, n * g.chunk_bytes, &sh.full[s.i]);
                 }
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&s_full[s], n * g.chunk_bytes + it.rows * have * kX);
-                    tma_bulk_g2s(stage, w + int64_t(c) * g.chunk_bytes, n * g.chunk_bytes, &s_full[s]);
+                if (waiting) {
+                    chain_wait();
+                    waiting = false;
                 }
-                __syncwarp();
-                if (lane < it.rows) tma_bulk_g2s(xs, x + int64_t(c) * kChunk * kX, have * kX, &s_full[s]);
-                if constexpr (X == XType::e4m3) {
-                    if (lane < it.rows) {
-                        for (int k = 0; k < n; ++k)
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(
-                                             smem_u32(stage + a.xs_at + (lane * kSlices + k) * 4)),
-                                         "l"(a.x_scale + int64_t(it.row + lane) * a.ld_xs + c + k)
-                                         : "memory");
+                if (elect_one()) {
+                    for (int h = 0; h < n; ++h) {
+                        const int chunk = c * a.step + h;
+                        tma_tile_g2s(stage + h * a.tile * TERMS * kChunk, &xmap, chunk * kChunk, it.row * TERMS, &sh.full[s.i]);
+                        if constexpr (TERMS == 1)
+                            tma_bulk_g2s(stage + a.f_at + h * a.tile * kFactBytes,
+                                         a.facts + (int64_t(chunk) * a.R + it.row) * (kFactBytes / 4), it.rows * kFactBytes,
+                                         &sh.full[s.i]);
                     }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&s_full[s]))
-                                 : "memory");
                 }
-                issued = max(issued, s + 1);
-                if (++s == a.stages) {
-                    s = 0;
-                    phase ^= 1;
-                }
+                __syncwarp();
+                issued = max(issued, s.i + 1);
+                s.next(a.stages);
             }
         }
+        if (waiting) chain_wait();  // this grid must not be done before the one that it did not wait for
         // no copy is left in flight when the CTA ends, whatever became of the consumers
-        for (int j = 0; j < a.stages; ++j)
-            if (j < issued) mbar_wait(&s_full[j], j < s ? phase : phase ^ 1, a.err);
+        for (int j = 0; j < issued; ++j) mbar_wait(&sh.full[j], j < s.i ? s.phase : s.phase ^ 1, a.err);
+    } else if (warp == kWarpMma) {
+        if (elect_one()) mma_role<TERMS, GROUPS>(a, sh, sp);
+    } else if (warp < kWarpOut) {
+        widen_role<GROUPS>(a, sh, sp);
     } else {
-        const int slice = warp / (4 / kRowTiles), row_tile = warp % (4 / kRowTiles) * kRowTiles;
-        int s = 0, turn = 0;
-        uint32_t phase = 0;
-        bool alive = true;
         // rows of no expert
-        {
-            const int used = s_row[g.E], lead = s_row[0];
-            const int64_t outside = int64_t(lead) + (a.R - used);
-            for (int64_t r = blockIdx.x; r < outside; r += gridDim.x) {
-                const int64_t row = r < lead ? r : r - lead + used;
-                const float zero[1] = {0.0f};
-                for (int n = threadIdx.x; n < g.out_n; n += kConsumers * 32)
-                    store_act<1>(a.out, a.out_dtype, row * a.ld_out + n, zero);
-            }
+        const int used = sh.row[g.E], lead = sh.row[0];
+        const int64_t outside = int64_t(lead) + (a.R - used);
+        for (int64_t r = blockIdx.x; r < outside; r += gridDim.x) {
+            const float zero[1] = {0.0f};
+            for (int n = int(threadIdx.x) - kWarpOut * 32; n < g.out_n; n += kOutSets * 128)
+                store_act<1>(a.out, a.out_dtype, (r < lead ? r : r - lead + used) * a.ld_out + n, zero);
         }
-        for (int64_t i = first; i < items; i += step, ++turn) {
-            const Item it = find_item(a, s_tile, s_row, i);
-            auto product = [&](auto tiles) {
-                constexpr int NT = decltype(tiles)::value;
-                float acc[kRowTiles][NT][4];
-#pragma unroll
-                for (int r = 0; r < kRowTiles; ++r)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        acc[r][t][0] = acc[r][t][1] = acc[r][t][2] = acc[r][t][3] = 0.0f;
-                for (int c = chunk0; alive && c < chunk1; c += kSlices) {
-                    alive = mbar_wait(&s_full[s], phase, a.err);
-                    const uint8_t* stage = s_ring + s * a.stage_bytes;
-                    if (alive && c + slice < chunk1)
-                        chunk_product<X, GROUPS, NT>(g, stage + slice * g.chunk_bytes,
-                                                     stage + a.x_at + slice * kChunk * kX,
-                                                     reinterpret_cast<const float*>(stage + a.xs_at) + slice, row_tile,
-                                                     lane, acc);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&s_empty[s]);
-                    if (++s == a.stages) {
-                        s = 0;
-                        phase ^= 1;
-                    }
-                }
-                const int n = row_tile * 16 + (lane >> 2), m = (lane & 3) * 2;
-#pragma unroll
-                for (int r = 0; r < kRowTiles; ++r) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float* p = s_slice + slice * values_cap + (t * 8 + m) * kRows + n + r * 16;
-                        p[0] = acc[r][t][0];
-                        p[kRows] = acc[r][t][1];
-                        p[8] = acc[r][t][2];
-                        p[kRows + 8] = acc[r][t][3];
-                    }
-                }
-            };
-            if (it.rows <= 8) product(std::integral_constant<int, 1>{});
-            else if (!WIDE || it.rows <= 16) product(std::integral_constant<int, 2>{});
-            else if constexpr (WIDE) product(std::integral_constant<int, 4>{});
-            consumer_sync();
-            // the slices' sums, and over a cluster the CTAs', in fixed order
-            const int values = it.rows * kRows;
-            auto slices = [&](int v) {
-                float y = s_slice[v];
-#pragma unroll
-                for (int k = 1; k < kSlices; ++k) y += s_slice[k * values_cap + v];
-                return y;
-            };
-            float* part = s_part + (turn & 1) * values_cap;
-            int v0 = 0, v1 = values;
-            if (a.ranks > 1) {
-                for (int v = threadIdx.x; v < values; v += kConsumers * 32) part[v] = slices(v);
-                consumer_sync();
-                // two barriers in turn: a fast CTA's arrival for the next item cannot count for this one
-                if (threadIdx.x < a.ranks) arrive_remote(&s_join[turn & 1], threadIdx.x);
-                if (alive) alive = wait_cluster(&s_join[turn & 1], (turn >> 1) & 1, a.err);
-                const int share = (it.rows + a.ranks - 1) / a.ranks;  // rows of x that this CTA writes
-                v0 = min(rank * share, it.rows) * kRows;
-                v1 = min(v0 + share * kRows, values);
-            }
-            const int per_block = g.swiglu ? kRows / 2 : kRows;
-            for (int v = v0 + int(threadIdx.x); v < v1; v += kConsumers * 32) {
-                const int n = v % kRows, col = it.block * per_block + n;
-                if (n >= per_block || col >= g.out_n) continue;
-                float y[1], gate = 0.0f;
-                if (a.ranks == 1) {
-                    y[0] = slices(v);
-                    if (g.swiglu) gate = slices(v + 32);
-                } else {
-                    y[0] = 0.0f;
-                    for (int r = 0; r < a.ranks; ++r) {
-                        y[0] += load_remote(part + v, r);
-                        if (g.swiglu) gate += load_remote(part + v + 32, r);
-                    }
-                }
-                if (g.swiglu) y[0] *= gate / (1.0f + expf(-gate));
-                store_act<1>(a.out, a.out_dtype, int64_t(it.row + v / kRows) * a.ld_out + col, y);
-            }
-            if (a.ranks == 1) consumer_sync();  // the slices are read before the next item's are written
-        }
+        out_role<TERMS, GROUPS>(a, sh, s_part, sp, rank);
     }
-    // no CTA of a cluster leaves while another may still read its sums or arrive on its barrier
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kWarpMma) tmem_dealloc(sh.tmem, 512);
+    // no CTA of a cluster leaves while another may still read its sums or arrive on its barriers
     if (a.ranks > 1) {
         __syncwarp();
-        asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+        cluster_barrier();
     }
 }
 
-// Rows of x of an item.  Taking more rows than an expert has costs shared memory (ring depth); taking
-// fewer runs its weights twice, the second time from L2.
-int choose_tile(int R, int E) {
+// Rows of x of an item.  A pass over an expert's weights costs the same for 1 row as for a tile of 8, and rows
+// that a tile has and the expert has not cost little: the tile holds about twice the mean, unless its
+// accumulators would leave tensor memory no second step.
+int choose_tile(int R, int E, int columns_a_row) {
     const int mean = (R + E - 1) / E;
-    return R <= 8 || mean <= 4 ? 8 : R <= 16 || mean <= 8 ? 16 : 32;
+    int tile = R <= 8 || mean <= 4 ? 8 : R <= 16 || mean <= 8 ? 16 : 32;
+    while (tile > 8 && tile * columns_a_row > kMostColumns) tile /= 2;
+    return tile;
 }
 
-// CTAs that share an item's k.  A wave of clusters takes (stages / ranks + a fixed cost) for each of its
+// CTAs that share an item's k.  A wave of clusters takes (steps / ranks + a fixed cost) for each of its
 // rounds; few items leave SMs idle unless k is split.
-int choose_ranks(int64_t items, int all_stages, int sms) {
+int choose_ranks(int64_t items, int steps, int sms) {
     int best = 1;
     double least = 0;
     for (int ranks = 1; ranks <= 8; ranks *= 2) {
         const int64_t slots = sms / ranks, rounds = (items + slots - 1) / slots;
-        const double cost = double(rounds) * ((all_stages + ranks - 1) / ranks + (ranks == 1 ? 2 : 4));
+        const double cost = double(rounds) * ((steps + ranks - 1) / ranks + (ranks == 1 ? 2 : 4));
         if (ranks == 1 || cost < least) {
             least = cost;
             best = ranks;
@@ -626,52 +868,104 @@ int choose_ranks(int64_t items, int all_stages, int sms) {
     return best;
 }
 
-template <XType X, int GROUPS, bool WIDE>
-cudaError_t launch_int4(Int4Args a, int sms, cudaStream_t stream) {
-    constexpr int kShared = WIDE ? 216 * 1024 : 103 * 1024;
-    sms *= WIDE ? 1 : 2;
-    a.x_at = kSlices * a.g.chunk_bytes;
-    a.xs_at = a.x_at + a.tile * x_pitch<X>();
-    a.stage_bytes = (a.xs_at + (X == XType::e4m3 ? a.tile * kSlices * 4 : 0) + 127) / 128 * 128;
-    const int all_stages = (a.g.chunks + kSlices - 1) / kSlices;
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+int64_t terms_bytes(const Geom& g, int terms, int64_t R) {
+    return (R * terms * g.chunks * kChunk + 255) / 256 * 256;
+}
+
+template <int TERMS, int GROUPS>
+int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
+    constexpr int kShared = 216 * 1024;
+    a.tile = choose_tile(a.R, a.g.E, TERMS * GROUPS);
+    a.d_cols = (a.tile * TERMS + 15) / 16 * 16;
+    // tensor memory: of a chunk, and once for a constant zero point
+    const int cols = kACols + (a.d_cols + (a.g.has_zero ? 8 : 0)) * GROUPS, once = a.g.has_zero ? 0 : 8;
+    for (a.step = kMaxStep; a.step > 1 && (512 - once) / (a.step * cols) < 2;) a.step /= 2;
+    a.bufs = (512 - once) / (a.step * cols);
+    if (a.bufs > kMaxBufs) a.bufs = kMaxBufs;
+    a.z_at = a.bufs * a.step * kACols;
+    a.d_at = a.z_at + (a.g.has_zero ? a.bufs * a.step * GROUPS * 8 : 8);
+    a.q_at = a.step * a.tile * TERMS * kChunk;
+    a.f_at = a.q_at + a.step * a.g.chunk_bytes;
+    a.stage_bytes = (a.f_at + (TERMS == 1 ? a.step * a.tile * kFactBytes : 0) + 1023) / 1024 * 1024;
     // experts with rows: at most every expert and every row; tiles of rows beyond one an expert
     const int64_t touched = a.R < a.g.E ? a.R : a.g.E;
     const int64_t most = (touched + a.R / a.tile) * a.g.blocks;
-    a.ranks = choose_ranks(a.R <= a.tile ? int64_t(a.g.blocks) * touched : most, all_stages, sms);
-    const int sums = (kSlices + (a.ranks > 1 ? 2 : 0)) * a.tile * kRows * 4;
+    a.ranks = choose_ranks(a.R <= a.tile ? int64_t(a.g.blocks) * touched : most, (a.g.chunks + a.step - 1) / a.step, sms);
+    const int sums = (a.ranks > 1 ? 2 : 1) * kOutSets * a.tile * kRows * 4;
     a.stages = (kShared - sums) / a.stage_bytes;
     if (a.stages > kMaxStages) a.stages = kMaxStages;
+    if (a.stages < 2 || a.bufs < 1) return set_last_error(CST_ERR_INVALID_ARG, "no room for a product of this shape");
     const int64_t clusters = most < sms / a.ranks ? most : sms / a.ranks;
-    auto kernel = int4_kernel<X, GROUPS, WIDE>;
+
+    CUtensorMap map;
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[2] = {cuuint64_t(a.g.chunks) * kChunk, cuuint64_t(a.R) * TERMS};
+    const cuuint64_t strides[1] = {dims[0]};
+    const cuuint32_t box[2] = {kChunk, cuuint32_t(a.tile * TERMS)}, steps[2] = {1, 1};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, workspace, dims, strides, box, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+
+    auto kernel = int4_kernel<TERMS, GROUPS>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(clusters * a.ranks));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = size_t(a.stages) * a.stage_bytes + sums;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.ranks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = a.ranks > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(clusters * a.ranks));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = size_t(a.stages) * a.stage_bytes + sums;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = a.ranks;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = a.ranks > 1 ? 2 : 1;
+        e = cudaLaunchKernelEx(&cfg, kernel, map, a);
+    }
+    if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "grouped_int4 launch failed: %s", cudaGetErrorString(e));
+    return CST_OK;
 }
 
-template <XType X, int GROUPS>
-cudaError_t launch_tile(Int4Args a, int sms, cudaStream_t s) {
-    a.tile = choose_tile(a.R, a.g.E);
-    return a.tile > 16 ? launch_int4<X, GROUPS, true>(a, sms, s) : launch_int4<X, GROUPS, false>(a, sms, s);
+template <int TERMS>
+int launch_terms(Int4Args a, const void* x, int x_dtype, int64_t ld_x, const float* x_scale, int64_t ld_xs,
+                 void* workspace, int sms, cudaStream_t s) {
+    float* facts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + terms_bytes(a.g, TERMS, a.R));
+    a.facts = facts;
+    const cudaError_t e = launch_chained(split_x_kernel<TERMS>, dim3(unsigned(a.R)), dim3(256), 0, s, x, x_dtype, ld_x,
+                                         x_scale, ld_xs, a.R, a.g.K, static_cast<uint8_t*>(workspace), facts);
+    if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "split_x launch failed: %s", cudaGetErrorString(e));
+    return a.g.group == 128  ? launch_int4<TERMS, 1>(a, workspace, sms, s)
+           : a.g.group == 64 ? launch_int4<TERMS, 2>(a, workspace, sms, s)
+                             : launch_int4<TERMS, 4>(a, workspace, sms, s);
 }
 
-template <XType X>
-cudaError_t launch_groups(const Int4Args& a, int sms, cudaStream_t s) {
-    return a.g.group == 128 ? launch_tile<X, 1>(a, sms, s)
-           : a.g.group == 64 ? launch_tile<X, 2>(a, sms, s)
-                             : launch_tile<X, 4>(a, sms, s);
+int terms_of(int x_dtype) { return x_dtype == CST_DTYPE_E4M3 ? 1 : x_dtype == CST_DTYPE_BF16 ? 2 : 3; }
+
+int check_x_dtype(int x_dtype) {
+    if (x_dtype != CST_DTYPE_FP16 && x_dtype != CST_DTYPE_BF16 && x_dtype != CST_DTYPE_E4M3)
+        return set_last_error(CST_ERR_INVALID_ARG, "x must be fp16, bf16 or e4m3, got dtype %d", x_dtype);
+    return CST_OK;
 }
 
 int check_weight(const cst_int4_weight* w) {
@@ -741,47 +1035,51 @@ extern "C" int cst_int4_device_error(const cst_int4_weight* w, void* data, void*
     return CST_OK;
 }
 
-extern "C" int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
-                                const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R,
-                                void* out, int32_t out_dtype, int64_t ld_out, void* stream) {
+extern "C" int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int32_t R, int64_t* bytes) {
     clear_last_error();
     if (const int rc = check_weight(w)) return rc;
+    if (const int rc = check_x_dtype(x_dtype)) return rc;
+    if (R < 0 || !bytes) return set_last_error(CST_ERR_INVALID_ARG, "R=%d must be >= 0 and bytes not null", R);
     const Geom g = make_geom(*w);
-    if (x_dtype != CST_DTYPE_FP16 && x_dtype != CST_DTYPE_BF16 && x_dtype != CST_DTYPE_E4M3)
-        return set_last_error(CST_ERR_INVALID_ARG, "x must be fp16, bf16 or e4m3, got dtype %d", x_dtype);
+    const int terms = terms_of(x_dtype);
+    *bytes = terms_bytes(g, terms, R) + int64_t(R) * (terms == 1 ? g.chunks * kFactBytes : 4);
+    return CST_OK;
+}
+
+extern "C" int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
+                                const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R,
+                                void* workspace, void* out, int32_t out_dtype, int64_t ld_out, void* stream) {
+    clear_last_error();
+    if (const int rc = check_weight(w)) return rc;
+    if (const int rc = check_x_dtype(x_dtype)) return rc;
+    const Geom g = make_geom(*w);
     if (out_dtype < CST_DTYPE_FP16 || out_dtype > CST_DTYPE_FP32)
         return set_last_error(CST_ERR_INVALID_ARG, "invalid out dtype %d", out_dtype);
     if ((x_dtype == CST_DTYPE_E4M3) != (x_scale != nullptr) && R > 0)
         return set_last_error(CST_ERR_INVALID_ARG, "x_scale goes with e4m3 rows, and only with them");
     if (!offsets && w->n_experts != 1)
         return set_last_error(CST_ERR_INVALID_ARG, "offsets are needed for %d experts", w->n_experts);
-    if (R < 0 || ld_x < w->k || ld_out < g.out_n || (x_scale && ld_x_scale < (w->k + 127) / 128))
-        return set_last_error(CST_ERR_INVALID_ARG, "R=%d must be >= 0 and no row stride below the row", R);
+    if (R < 0 || R > (1 << 28) || ld_x < w->k || ld_out < g.out_n || (x_scale && ld_x_scale < (w->k + 127) / 128))
+        return set_last_error(CST_ERR_INVALID_ARG, "R=%d must be in [0, 2^28] and no row stride below the row", R);
     if (R == 0) return CST_OK;
-    if (!data || !x || !out) return set_last_error(CST_ERR_INVALID_ARG, "null data, x or out");
-    if (!rows_aligned16(x, ld_x, act_size(x_dtype)) || (reinterpret_cast<uintptr_t>(data) & 15u))
-        return set_last_error(CST_ERR_INVALID_ARG, "data and every row of x must be 16-byte aligned");
+    if (!data || !x || !out || !workspace)
+        return set_last_error(CST_ERR_INVALID_ARG, "null data, x, workspace or out");
+    if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(workspace)) & 15u))
+        return set_last_error(CST_ERR_INVALID_ARG, "data and workspace must be 16-byte aligned");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "cannot query the SM count: %s", cudaGetErrorString(e));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     Int4Args a{};
     a.g = g;
     a.data = static_cast<const uint8_t*>(data);
-    a.x = static_cast<const uint8_t*>(x);
-    a.ld_x = ld_x * act_size(x_dtype);
-    a.x_scale = x_scale;
-    a.ld_xs = ld_x_scale;
     a.offsets = offsets;
     a.R = R;
     a.out = out;
     a.out_dtype = out_dtype;
     a.ld_out = ld_out;
     a.err = reinterpret_cast<int*>(static_cast<uint8_t*>(data) + g.expert_bytes() * g.E);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    e = x_dtype == CST_DTYPE_BF16   ? launch_groups<XType::bf16>(a, sms, s)
-        : x_dtype == CST_DTYPE_FP16 ? launch_groups<XType::f16>(a, sms, s)
-                                    : launch_groups<XType::e4m3>(a, sms, s);
-    if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "grouped_int4 launch failed: %s", cudaGetErrorString(e));
-    return CST_OK;
+    auto launch = x_dtype == CST_DTYPE_E4M3 ? launch_terms<1> : x_dtype == CST_DTYPE_BF16 ? launch_terms<2> : launch_terms<3>;
+    return launch(a, x, x_dtype, ld_x, x_scale, ld_x_scale, workspace, sms, s);
 }

@@ -160,15 +160,16 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
         raise RuntimeError(f"out must be contiguous [{R}, {w.out_features}] on the device of x")
     ot = dtype_code(out.dtype)
     x, ldx = _rows(x)
-    size = x.element_size()
-    if x.data_ptr() % 16 or ldx * size % 16:  # the kernel copies whole 16-byte pieces of a row
-        x, ldx = x.clone(memory_format=torch.contiguous_format), K
     lds = 0
     if x_scale is not None:
         x_scale, lds = _rows(x_scale)
+    size = ctypes.c_int64()
+    check(_lib.lib.cst_int4_workspace(w._ref, xt, R, ctypes.byref(size)))
+    room = torch.empty(size.value, dtype=torch.uint8, device=dev)
     with _on(dev):
         check(_lib.lib.cst_grouped_int4(w._ref, w.data.data_ptr(), x.data_ptr(), xt, ldx, _ptr(x_scale), lds,
-                                        _ptr(offsets), R, out.data_ptr(), ot, w.out_features, _stream(dev)))
+                                        _ptr(offsets), R, room.data_ptr(), out.data_ptr(), ot, w.out_features,
+                                        _stream(dev)))
     return out
 
 

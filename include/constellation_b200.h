@@ -322,16 +322,20 @@ int cst_int4_bytes(const cst_int4_weight* w, int64_t* bytes);
  * is not laid out is all zero.  Load-time, stream-ordered. */
 int cst_int4_pack(const cst_int4_weight* w, int32_t first, int32_t count, const uint8_t* q, const void* scale,
                   const uint8_t* zero, void* data, void* stream);
+/* Bytes of the workspace of a product of R rows of x_dtype. */
+int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int32_t R, int64_t* bytes);
 /* out[r] = W[e] x[r] for the rows r in [offsets[e], offsets[e + 1]) of each expert (device int32
  * [n_experts + 1], ascending; the kernel clamps them to [0, R] and to ascending order), zero for the
  * rows outside; offsets NULL: one expert, every row.
- *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise);
- *        rows 16-byte aligned (base and stride)
+ *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise)
+ *   workspace  cst_int4_workspace bytes, 16-byte aligned, of this call alone until it is done
  *   out  [R, n] (n / 2 with swiglu) in out_dtype (fp16, bf16, fp32)
- * fp32 sums of exact products, one rounding.  `data` is only read, but for its error word. */
+ * x enters the products as 8-bit terms that hold it exactly but for what is below 2^-21 (bf16) or
+ * 2^-25 (fp16) of the largest |x| of its row; sums are fp32, with one rounding.
+ * An infinity in a row of x makes the row's results NaN.  `data` is only read, but for its error word. */
 int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
-                     const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* out,
-                     int32_t out_dtype, int64_t ld_out, void* stream);
+                     const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* workspace,
+                     void* out, int32_t out_dtype, int64_t ld_out, void* stream);
 /* Waits for `stream`, then returns CST_OK or CST_ERR_DEVICE_TIMEOUT if a bounded wait of a product
  * with this weight gave up since the last call (and clears the word). */
 int cst_int4_device_error(const cst_int4_weight* w, void* data, void* stream);

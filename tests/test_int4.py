@@ -453,9 +453,9 @@ def test_refusals_without_a_device():
         return ctypes.byref(_lib.CstInt4Weight(E, n, k, group, st, z, sw))
 
     size = ctypes.c_int64()
-    assert L.cst_int4_bytes(weight(), ctypes.byref(size)) == 0 and size.value == 4096 + 64 * 2 + 256
-    assert L.cst_int4_bytes(weight(E=3, n=65, k=160, group=32, st=3, z=1), ctypes.byref(size)) == 0
-    assert size.value == 3 * 2 * 2 * (4096 + 4 * 64 * 4 + 4 * 64) + 256
+    assert L.cst_int4_bytes(weight(), ctypes.byref(size)) == 0 and size.value == 8192 + 128 * 2 + 256
+    assert L.cst_int4_bytes(weight(E=3, n=129, k=160, group=32, st=3, z=1), ctypes.byref(size)) == 0
+    assert size.value == 3 * 2 * 2 * (8192 + 4 * 128 * 4 + 4 * 128) + 256
     for kw in (dict(E=0), dict(E=1025), dict(n=0), dict(k=0), dict(group=16), dict(k=130), dict(st=4), dict(n=3, sw=1),
                dict(n=1 << 21)):
         assert L.cst_int4_bytes(weight(**kw), ctypes.byref(size)) == BAD, kw
@@ -468,11 +468,17 @@ def test_refusals_without_a_device():
     assert L.cst_int4_pack(weight(), 0, 0, None, None, None, None, None) == _lib.CST_OK
     assert L.cst_int4_device_error(weight(), None, None) == BAD
 
-    def call(w=None, data=P, x=P, xt=2, ldx=128, xs=None, lds=1, off=P, R=1, out=P, ot=2, ldo=64):
-        return L.cst_grouped_int4(w or weight(), data, x, xt, ldx, xs, lds, off, R, out, ot, ldo, None)
+    assert L.cst_int4_workspace(weight(), 2, 3, ctypes.byref(size)) == 0 and size.value == 768 + 3 * 4
+    assert L.cst_int4_workspace(weight(), 4, 3, ctypes.byref(size)) == 0 and size.value == 512 + 3 * 16
+    for a in ((weight(), 3, 1), (weight(), 2, -1), (weight(group=16), 2, 1)):
+        assert L.cst_int4_workspace(*a, ctypes.byref(size)) == BAD
+    assert L.cst_int4_workspace(weight(), 2, 1, None) == BAD
+
+    def call(w=None, data=P, x=P, xt=2, ldx=128, xs=None, lds=1, off=P, R=1, ws=P, out=P, ot=2, ldo=64):
+        return L.cst_grouped_int4(w or weight(), data, x, xt, ldx, xs, lds, off, R, ws, out, ot, ldo, None)
 
     assert call(data=None, x=None, out=None, R=0) == _lib.CST_OK
     for kw in (dict(xt=3), dict(xt=4), dict(xs=P), dict(ot=4), dict(ldx=127), dict(ldo=63), dict(R=-1), dict(x=None),
                dict(out=None), dict(data=None), dict(w=weight(E=2), off=None), dict(xt=4, xs=P, lds=0),
-               dict(x=8), dict(ldx=129)):
+               dict(ws=None), dict(ws=8), dict(data=8), dict(R=(1 << 28) + 1)):
         assert call(**kw) == BAD, kw
