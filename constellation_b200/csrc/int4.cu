@@ -216,22 +216,22 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
 // ---- the product ---------------------------------------------------------------------------
 // One persistent CTA per SM walks items (row tile of an expert, block of 128 weight rows); the
 // CTAs of a cluster split an item's k.  Per step of up to four chunks of 128 k:
-//   warp 0     producer: one bulk copy of the packed weights with their scales (8.4 KB a chunk), TMA tiles of
-//              x's terms [tile * TERMS][128 k], swizzled as the matrix unit reads them (and for e4m3 the
-//              rows' scales), into a ring;
-//   warps 2..  four wideners: each thread owns a weight row, turns its 64 packed bytes into 128 e4m3
+//   warp 0     one lane is the producer: one bulk copy of the packed weights with their scales (8.4 KB a
+//              chunk) and one TMA box of x's terms [step][tile * TERMS][128 k], swizzled as the matrix unit
+//              reads them (and for e4m3 the rows' scales), into a ring;
+//   warps 2..  wideners, two sets of four: each thread owns a weight row, turns its 64 packed bytes into 128 e4m3
 //              numbers with 48 logic operations and stores them to tensor memory, where they are the matrix
 //              product's A operand (and the row's zero points, if there are any);
 //   warp 1     one lane issues the tcgen05 products, a fresh fp32 accumulator for each group;
-//   the last   four output warps: each thread owns a weight row of the accumulators:
+//   the last   output warps, as many sets: each thread owns a weight row of the accumulators:
 //              acc[t] += 2^9 scale * (D1[t] + D2[t] / 16 + D3[t] / 256), and at the end of an item the results.
 // So each weight byte is read once from HBM and once from shared memory, and never goes back there.
 
 constexpr int kMaxStages = 12;
 constexpr int kMaxStep = 4;                     // chunks of a step, which the roles hand on at a time
-constexpr int kWidenSets = 1, kOutSets = 1;     // sets of 4 warps, which take the chunks of a step in turn
-constexpr int kWarpMma = 1, kWarpWiden = 2, kWarpOut = kWarpWiden + 4 * kWidenSets;
-constexpr int kThreads = (kWarpOut + 4 * kOutSets) * 32;
+constexpr int kSets = 2;                        // sets of 4 wideners and of 4 output warps, which take the steps in turn
+constexpr int kWarpMma = 1, kWarpWiden = 2, kWarpOut = kWarpWiden + 4 * kSets;
+constexpr int kThreads = (kWarpOut + 4 * kSets) * 32;
 constexpr int kMaxBufs = 4;                     // steps in tensor memory
 constexpr int kACols = kChunk / 4;              // columns of A: [128 rows][128 k] of 8 bits
 constexpr int kMostColumns = 512 / 2 - kACols - 32;  // accumulator columns of a chunk with which two steps fit
@@ -263,11 +263,12 @@ __device__ __forceinline__ float scale_at(const uint8_t* scales, int dtype, int 
     return __half2float(reinterpret_cast<const __half*>(scales)[s]);
 }
 
-__device__ __forceinline__ void tma_tile_g2s(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+// x's terms of rows from y and chunks from z, all 128 columns of them.
+__device__ __forceinline__ void tma_box_g2s(void* dst, const CUtensorMap* map, int y, int z, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
             smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        "l"(map), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -488,6 +489,47 @@ struct Span {
     int step0, step1;
 };
 
+// One elected lane.  A step is one bulk copy of its chunks and one TMA box of x's terms for all of them.
+template <int TERMS>
+__device__ __forceinline__ void producer_role(const Int4Args& a, Shared& sh, const CUtensorMap& xmap, const Span& sp) {
+    Ring s;
+    int issued = 0;
+    bool waiting = true;
+    const uint32_t x_bytes = uint32_t(a.step * a.tile * TERMS * kChunk);
+    for (int64_t i = sp.first; i < sp.items; i += sp.step) {
+        const Item it = find_item(a, sh.tile, sh.row, i);
+        const uint8_t* w = a.data + it.expert * a.g.expert_bytes() +
+                           (int64_t(it.block) * a.g.chunks + int64_t(sp.step0) * a.step) * a.g.chunk_bytes;
+        const int x_row = it.row * TERMS;
+        for (int c = sp.step0; c < sp.step1; ++c) {
+            if (!lane_wait(&sh.empty[s.i], s.phase ^ 1, a.err)) goto out;
+            uint8_t* stage = s_ring + s.i * a.stage_bytes;
+            const int n = min(a.step, a.g.chunks - c * a.step);
+            const uint32_t w_bytes = uint32_t(n * a.g.chunk_bytes);
+            // a TMA box always counts whole: what lies past the rows and chunks arrives as zeros
+            mbar_arrive_expect_tx(&sh.full[s.i], w_bytes + x_bytes + (TERMS == 1 ? n * it.rows * kFactBytes : 0));
+            tma_bulk_g2s(stage + a.q_at, w, w_bytes, &sh.full[s.i]);
+            w += w_bytes;
+            if (waiting) {
+                chain_wait();
+                waiting = false;
+            }
+            tma_box_g2s(stage, &xmap, x_row, c * a.step, &sh.full[s.i]);
+            if constexpr (TERMS == 1)
+                for (int h = 0; h < n; ++h)
+                    tma_bulk_g2s(stage + a.f_at + h * a.tile * kFactBytes,
+                                 a.facts + (int64_t(c * a.step + h) * a.R + it.row) * (kFactBytes / 4),
+                                 it.rows * kFactBytes, &sh.full[s.i]);
+            issued = max(issued, s.i + 1);
+            s.next(a.stages);
+        }
+    }
+out:
+    if (waiting) chain_wait();  // this grid must not be done before the one that it did not wait for
+    // no copy is left in flight when the CTA ends, whatever became of the consumers
+    for (int j = 0; j < issued; ++j) lane_wait(&sh.full[j], j < s.i ? s.phase : s.phase ^ 1, a.err);
+}
+
 template <int GROUPS>
 __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const Span& sp) {
     const int warp = (int(threadIdx.x) >> 5) - kWarpWiden, lane = threadIdx.x & 31, set = warp >> 2;
@@ -498,15 +540,21 @@ __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const 
         if (set == 0) tmem_fill8(lanes + a.z_at, 0x88888888u);
     }
     Ring s, b;
+    int turn = set;
     for (int64_t i = sp.first; i < sp.items; i += sp.step) {
-        for (int c = sp.step0; c < sp.step1; ++c) {
+        for (int c = sp.step0; c < sp.step1; ++c, s.next(a.stages), b.next(a.bufs)) {
+            if (turn != 0) {
+                --turn;
+                continue;
+            }
+            turn = kSets - 1;
             if (!warp_wait(&sh.full[s.i], s.phase, a.err) || !warp_wait(&sh.done[b.i], b.phase ^ 1, a.err)) return;
             tc_fence_after();
-            const uint8_t* chunk = s_ring + s.i * a.stage_bytes + a.q_at + set * a.g.chunk_bytes + row * 16;
-            uint32_t dst = lanes + (b.i * a.step + set) * kACols;
+            const uint8_t* chunk = s_ring + s.i * a.stage_bytes + a.q_at + row * 16;
+            uint32_t dst = lanes + b.i * a.step * kACols;
             const int n = min(a.step, a.g.chunks - c * a.step);
 #pragma unroll 1
-            for (int h = set; h < n; h += kWidenSets, chunk += kWidenSets * a.g.chunk_bytes, dst += kWidenSets * kACols) {
+            for (int h = 0; h < n; ++h, chunk += a.g.chunk_bytes, dst += kACols) {
                 uint32_t v[32];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {  // 32 k
@@ -534,8 +582,6 @@ __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const 
                 mbar_arrive(&sh.ready[b.i]);
                 mbar_arrive(&sh.empty[s.i]);
             }
-            s.next(a.stages);
-            b.next(a.bufs);
         }
     }
 }
@@ -543,13 +589,14 @@ __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const 
 // One elected lane.  The operands of an instruction come from uniform registers: under an elected
 // lane, with addresses that are sums of a base and constants, a 128 x 16 x 16 product takes 11 cycles to issue;
 // through a lane that the compiler does not know to be alone it took 160.
-template <int TERMS, int GROUPS>
+template <int TERMS, int GROUPS, int TILE, bool ZERO>
 __device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Span& sp) {
+    constexpr uint32_t kD = (TILE * TERMS + 15) / 16 * 16;  // columns of an accumulator
+    constexpr uint32_t kX = TILE * TERMS * kChunk / 16;     // bytes of x of a chunk, over 16
     Ring s, b;
     int used = 0;
     const uint64_t x0 = umma_desc_sw128(smem_u32(s_ring));
-    const uint32_t x_step = uint32_t(a.stage_bytes) >> 4, x_chunk = uint32_t(a.tile * TERMS) * 8;  // in 16 bytes
-    const uint32_t d_step = uint32_t(a.step * GROUPS * a.d_cols), z_group = a.g.has_zero ? 8 : 0;
+    const uint32_t x_step = uint32_t(a.stage_bytes) >> 4;
     for (int64_t i = sp.first; i < sp.items; i += sp.step) {
         const Item it = find_item(a, sh.tile, sh.row, i);
         const uint32_t idesc = umma_idesc_e4m3(128, (it.rows * TERMS + 15) / 16 * 16);
@@ -558,18 +605,18 @@ __device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Sp
             if (!lane_wait(&sh.ready[b.i], b.phase, a.err)) goto out;
             tc_fence_after();
             const uint64_t x = x0 + uint64_t(uint32_t(s.i) * x_step);
-            const uint32_t w = uint32_t(b.i) * (a.step * kACols), d = uint32_t(a.d_at) + uint32_t(b.i) * d_step;
-            const uint32_t z = uint32_t(a.z_at) + uint32_t(b.i * a.step * GROUPS) * z_group;
+            const uint32_t w = uint32_t(b.i * a.step) * kACols, d = uint32_t(a.d_at) + uint32_t(b.i * a.step * GROUPS) * kD;
+            const uint32_t z = uint32_t(a.z_at) + (ZERO ? uint32_t(b.i * a.step * GROUPS) * 8 : 0);
             const int n = min(a.step, a.g.chunks - c * a.step);
 #pragma unroll
             for (int h = 0; h < kMaxStep; ++h) {
                 if (h >= n) break;
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {  // 32 k
-                    const int g = h * GROUPS + ks / (4 / GROUPS);
-                    const uint64_t xk = x + uint32_t(h) * x_chunk + ks * 2;
-                    tc_mma_ts(d + uint32_t(g) * a.d_cols, w + h * kACols + ks * 8, xk, idesc, ks % (4 / GROUPS) > 0);
-                    tc_mma_ts(d + uint32_t(g) * a.d_cols, z + uint32_t(g) * z_group, xk, idesc, true);
+                    const uint32_t g = h * GROUPS + ks / (4 / GROUPS);
+                    const uint64_t xk = x + h * kX + ks * 2;
+                    tc_mma_ts(d + g * kD, w + h * kACols + ks * 8, xk, idesc, ks % (4 / GROUPS) > 0);
+                    tc_mma_ts(d + g * kD, ZERO ? z + g * 8 : z, xk, idesc, true);
                 }
             }
             tc_commit(&sh.done[b.i]);
@@ -591,25 +638,31 @@ __device__ __forceinline__ void load_columns(uint32_t d, uint32_t (&v)[N]) {
     if constexpr (N % 16) tmem_ld8(d + N - 8, v + N - 8);
 }
 
-// One item: the sums of ROWS rows of x over the chunks of this set of output warps, for this thread's weight
+// One item: the sums of ROWS rows of x over the steps of this set of output warps, for this thread's weight
 // row.
 template <int TERMS, int GROUPS, int ROWS>
-__device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, int set, int row,
-                                           uint32_t lanes, Ring& s, Ring& b, float (&acc)[ROWS]) {
-    constexpr int kAt = ROWS * TERMS <= 32 ? ROWS : 32 / TERMS / 8 * 8;  // rows whose columns are in registers at a time
-    constexpr int kGo = kOutSets == 1 && kAt == ROWS ? 32 / (kAt * TERMS) : 1;
+__device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, int row, uint32_t lanes,
+                                           Ring& s, Ring& b, int& turn, float (&acc)[ROWS]) {
+    // rows whose columns are in registers at a time
+    constexpr int kCols = 16, kFit = kCols / TERMS / 8 * 8 > 8 ? kCols / TERMS / 8 * 8 : 8;
+    constexpr int kAt = ROWS < kFit ? ROWS : kFit, kGo = kAt == ROWS && kAt * TERMS <= kCols ? kCols / (kAt * TERMS) : 1;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) acc[t] = 0.0f;
-    for (int c = sp.step0; c < sp.step1; ++c) {
+    for (int c = sp.step0; c < sp.step1; ++c, s.next(a.stages), b.next(a.bufs)) {
+        if (turn != 0) {
+            --turn;
+            continue;
+        }
+        turn = kSets - 1;
         if (!warp_wait(&sh.done[b.i], b.phase, a.err)) return false;
         tc_fence_after();
         const uint8_t* stage = s_ring + s.i * a.stage_bytes;
         const int n = min(a.step, a.g.chunks - c * a.step) * GROUPS;  // accumulators of the step
-        uint32_t d = a.d_at + lanes + (b.i * a.step + set) * GROUPS * a.d_cols;
+        uint32_t d = a.d_at + lanes + b.i * a.step * GROUPS * a.d_cols;
         // (chunk, group) pieces, kGo of them at a time while their columns fit in registers
 #pragma unroll 1
-        for (int p = set * GROUPS; p < n;) {
+        for (int p = 0; p < n; p += kGo, d += kGo * a.d_cols) {
             uint32_t v[kGo][kAt * TERMS];
             float scale[kGo];
 #pragma unroll
@@ -641,10 +694,6 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
                     }
                 }
             }
-            // on to the next piece, or over the other sets' chunks
-            const int go = kOutSets == 1 ? kGo : p % GROUPS == GROUPS - 1 ? (kOutSets - 1) * GROUPS + 1 : 1;
-            p += go;
-            d += go * a.d_cols;
         }
         tc_fence_before();
         __syncwarp();
@@ -652,8 +701,6 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
             mbar_arrive(&sh.ready[b.i]);
             mbar_arrive(&sh.empty[s.i]);
         }
-        s.next(a.stages);
-        b.next(a.bufs);
     }
     return true;
 }
@@ -672,25 +719,26 @@ __device__ __forceinline__ void write_out(const Int4Args& a, const Item& it, int
         store_act<1>(a.out, a.out_dtype, int64_t(it.row + t) * a.ld_out + col, v);
 }
 
-__device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kOutSets * 128) : "memory"); }
+__device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kSets * 128) : "memory"); }
 
 template <int TERMS, int GROUPS>
 __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s_part, const Span& sp, int rank) {
     const int lane = threadIdx.x & 31, quarter = (int(threadIdx.x) >> 5) & 3, row = quarter * 32 + lane;
     const int set = ((int(threadIdx.x) >> 5) - kWarpOut) >> 2, size = a.tile * kRows;
+    int wait_turns = set;  // steps until this set's next
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     Ring s, b;
     bool alive = true;
     uint32_t turn = 0;
-    if (lane == 0)  // no accumulators to take before the first products
+    if (lane == 0 && set == 0)  // no accumulators to take before the first products
         for (int j = 0; j < a.bufs; ++j) mbar_arrive(&sh.ready[j]);
     for (int64_t i = sp.first; i < sp.items; i += sp.step, ++turn) {
         const Item it = find_item(a, sh.tile, sh.row, i);
-        float* part = s_part + (a.ranks > 1 ? (turn & 1) * kOutSets * size : 0);  // [set][row of x][weight row]
+        float* part = s_part + (a.ranks > 1 ? (turn & 1) * kSets * size : 0);  // [set][row of x][weight row]
         auto item = [&](auto rows) {
             constexpr int ROWS = decltype(rows)::value;
             float acc[ROWS];
-            alive = alive && accumulate<TERMS, GROUPS, ROWS>(a, sh, sp, set, row, lanes, s, b, acc);
+            alive = alive && accumulate<TERMS, GROUPS, ROWS>(a, sh, sp, row, lanes, s, b, wait_turns, acc);
 #pragma unroll
             for (int t = 0; t < ROWS; ++t) part[set * size + t * kRows + row] = acc[t];
         };
@@ -700,7 +748,7 @@ __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s
         // Lane t has the scale of row t.  (The products above have read x's terms, so it is written.)
         const float scale = TERMS > 1 && lane < it.rows ? __ldcg(a.facts + it.row + lane) : 1.0f;
         int t0 = 0, t1 = it.rows;
-        if (a.ranks > 1 || kOutSets > 1) output_sync();
+        output_sync();
         if (a.ranks > 1) {
             // the CTAs' sums over the cluster, in order; two barriers in turn, so that a fast CTA's arrival
             // for the next item cannot count for this one
@@ -712,21 +760,21 @@ __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s
             t1 = min(t0 + share, it.rows);
         }
 #pragma unroll 4
-        for (int t = t0 + set; t < t1; t += kOutSets) {
+        for (int t = t0 + set; t < t1; t += kSets) {
             float y = 0.0f;
             if (a.ranks == 1) {
 #pragma unroll
-                for (int h = 0; h < kOutSets; ++h) y += part[h * size + t * kRows + row];
+                for (int h = 0; h < kSets; ++h) y += part[h * size + t * kRows + row];
             } else {
                 for (int r = 0; r < a.ranks; ++r)
 #pragma unroll
-                    for (int h = 0; h < kOutSets; ++h) y += load_remote(part + h * size + t * kRows + row, r);
+                    for (int h = 0; h < kSets; ++h) y += load_remote(part + h * size + t * kRows + row, r);
             }
             if constexpr (TERMS > 1) y *= __shfl_sync(0xffffffffu, scale, t);
             write_out(a, it, row, t, y);
         }
         // the sums are read before the next item's are written
-        if (a.ranks == 1 && kOutSets > 1) output_sync();
+        if (a.ranks == 1) output_sync();
     }
 }
 
@@ -742,10 +790,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&sh.full[s], 1);  // the producer's arrival with the bytes to come
-            mbar_init(&sh.empty[s], 4 * (kWidenSets + kOutSets));  // the output warps arrive after the products
+            mbar_init(&sh.empty[s], 4 + 4);  // a set of wideners; a set of output warps, after the products
         }
         for (int b = 0; b < a.bufs; ++b) {
-            mbar_init(&sh.ready[b], 4 * (kWidenSets + kOutSets));
+            mbar_init(&sh.ready[b], 4 + 4);
             mbar_init(&sh.done[b], 1);
         }
         mbar_init(&sh.join[0], a.ranks);
@@ -775,48 +823,20 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
     sp.step1 = min(sp.step0 + per, steps);
 
     if (warp == 0) {
-        Ring s;
-        int issued = 0;
-        bool alive = true, waiting = true;
-        for (int64_t i = sp.first; alive && i < sp.items; i += sp.step) {
-            const Item it = find_item(a, sh.tile, sh.row, i);
-            const uint8_t* w = a.data + it.expert * g.expert_bytes() + int64_t(it.block) * g.chunks * g.chunk_bytes;
-            for (int c = sp.step0; c < sp.step1; ++c) {
-                alive = warp_wait(&sh.empty[s.i], s.phase ^ 1, a.err);
-                if (!alive) break;
-                uint8_t* stage = s_ring + s.i * a.stage_bytes;
-                const int n = min(a.step, g.chunks - c * a.step);
-                if (elect_one()) {
-                    // a TMA tile always counts whole: what lies past the rows arrives as zeros
-                    mbar_arrive_expect_tx(&sh.full[s.i],
-                                          n * (g.chunk_bytes + a.tile * TERMS * kChunk + (TERMS == 1 ? it.rows * kFactBytes : 0)));
-                    tma_bulk_g2s(stage + a.q_at, w + int64_t(c) * a.step * g.chunk_bytes, n * g.chunk_bytes, &sh.full[s.i]);
-                }
-                __syncwarp();
-                if (waiting) {
-                    chain_wait();
-                    waiting = false;
-                }
-                if (elect_one()) {
-                    for (int h = 0; h < n; ++h) {
-                        const int chunk = c * a.step + h;
-                        tma_tile_g2s(stage + h * a.tile * TERMS * kChunk, &xmap, chunk * kChunk, it.row * TERMS, &sh.full[s.i]);
-                        if constexpr (TERMS == 1)
-                            tma_bulk_g2s(stage + a.f_at + h * a.tile * kFactBytes,
-                                         a.facts + (int64_t(chunk) * a.R + it.row) * (kFactBytes / 4), it.rows * kFactBytes,
-                                         &sh.full[s.i]);
-                    }
-                }
-                __syncwarp();
-                issued = max(issued, s.i + 1);
-                s.next(a.stages);
+        if (elect_one()) producer_role<TERMS>(a, sh, xmap, sp);
+    } else if (warp == kWarpMma) {
+        if (elect_one()) {
+            if (a.tile == 8) {
+                if (g.has_zero) mma_role<TERMS, GROUPS, 8, true>(a, sh, sp);
+                else mma_role<TERMS, GROUPS, 8, false>(a, sh, sp);
+            } else if (a.tile == 16) {
+                if (g.has_zero) mma_role<TERMS, GROUPS, 16, true>(a, sh, sp);
+                else mma_role<TERMS, GROUPS, 16, false>(a, sh, sp);
+            } else {
+                if (g.has_zero) mma_role<TERMS, GROUPS, 32, true>(a, sh, sp);
+                else mma_role<TERMS, GROUPS, 32, false>(a, sh, sp);
             }
         }
-        if (waiting) chain_wait();  // this grid must not be done before the one that it did not wait for
-        // no copy is left in flight when the CTA ends, whatever became of the consumers
-        for (int j = 0; j < issued; ++j) mbar_wait(&sh.full[j], j < s.i ? s.phase : s.phase ^ 1, a.err);
-    } else if (warp == kWarpMma) {
-        if (elect_one()) mma_role<TERMS, GROUPS>(a, sh, sp);
     } else if (warp < kWarpOut) {
         widen_role<GROUPS>(a, sh, sp);
     } else {
@@ -825,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
         const int64_t outside = int64_t(lead) + (a.R - used);
         for (int64_t r = blockIdx.x; r < outside; r += gridDim.x) {
             const float zero[1] = {0.0f};
-            for (int n = int(threadIdx.x) - kWarpOut * 32; n < g.out_n; n += kOutSets * 128)
+            for (int n = int(threadIdx.x) - kWarpOut * 32; n < g.out_n; n += kSets * 128)
                 store_act<1>(a.out, a.out_dtype, (r < lead ? r : r - lead + used) * a.ld_out + n, zero);
         }
         out_role<TERMS, GROUPS>(a, sh, s_part, sp, rank);
@@ -896,7 +916,7 @@ int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
     a.d_cols = (a.tile * TERMS + 15) / 16 * 16;
     // tensor memory: of a chunk, and once for a constant zero point
     const int cols = kACols + (a.d_cols + (a.g.has_zero ? 8 : 0)) * GROUPS, once = a.g.has_zero ? 0 : 8;
-    for (a.step = kMaxStep; a.step > 1 && (512 - once) / (a.step * cols) < 2;) a.step /= 2;
+    for (a.step = kMaxStep; a.step > 1 && (512 - once) / (a.step * cols) < 2;) --a.step;
     a.bufs = (512 - once) / (a.step * cols);
     if (a.bufs > kMaxBufs) a.bufs = kMaxBufs;
     a.z_at = a.bufs * a.step * kACols;
@@ -908,7 +928,7 @@ int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
     const int64_t touched = a.R < a.g.E ? a.R : a.g.E;
     const int64_t most = (touched + a.R / a.tile) * a.g.blocks;
     a.ranks = choose_ranks(a.R <= a.tile ? int64_t(a.g.blocks) * touched : most, (a.g.chunks + a.step - 1) / a.step, sms);
-    const int sums = (a.ranks > 1 ? 2 : 1) * kOutSets * a.tile * kRows * 4;
+    const int sums = (a.ranks > 1 ? 2 : 1) * kSets * a.tile * kRows * 4;
     a.stages = (kShared - sums) / a.stage_bytes;
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     if (a.stages < 2 || a.bufs < 1) return set_last_error(CST_ERR_INVALID_ARG, "no room for a product of this shape");
@@ -917,10 +937,11 @@ int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
     CUtensorMap map;
     const EncodeTiled encode = encode_tiled();
     if (!encode) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[2] = {cuuint64_t(a.g.chunks) * kChunk, cuuint64_t(a.R) * TERMS};
-    const cuuint64_t strides[1] = {dims[0]};
-    const cuuint32_t box[2] = {kChunk, cuuint32_t(a.tile * TERMS)}, steps[2] = {1, 1};
-    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, workspace, dims, strides, box, steps,
+    // [chunk][row and term][128 columns of the chunk]
+    const cuuint64_t dims[3] = {kChunk, cuuint64_t(a.R) * TERMS, cuuint64_t(a.g.chunks)};
+    const cuuint64_t strides[2] = {dims[2] * kChunk, kChunk};
+    const cuuint32_t box[3] = {kChunk, cuuint32_t(a.tile * TERMS), cuuint32_t(a.step)}, steps[3] = {1, 1, 1};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, workspace, dims, strides, box, steps,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
