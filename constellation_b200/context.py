@@ -68,8 +68,16 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+try:  # the address alone, without a stream object
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:  # pragma: no cover
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device``, which has an index."""
+    return _raw_stream(device.index)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *,
@@ -137,7 +145,7 @@ def _add_rms_norm(what, x, residual, weight, eps, sum_out, out, out_dtype):
         given = residual
         residual, ldr = _rows(residual)
         if sum_out is None:
-            sum_out = torch.empty((T, H), dtype=given.dtype, device=dev)
+            sum_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
         elif sum_out.dtype != given.dtype or sum_out.shape != x.shape or sum_out.device != dev:
             raise RuntimeError("sum_out must have the shape, type and device of residual")
         lds = _out_rows("sum_out", sum_out)
@@ -146,13 +154,13 @@ def _add_rms_norm(what, x, residual, weight, eps, sum_out, out, out_dtype):
     scale = None
     if out_dtype is None:
         if out is None:
-            out = torch.empty((T, H), dtype=x.dtype, device=dev)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out.shape != x.shape or out.device != dev:
             raise RuntimeError("out must have the shape and device of x")
         ot = dtype_code(out.dtype)
         ldo = _out_rows("out", out)
     else:
-        out = torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev)
+        out = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
         scale = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=dev)
         ot, ldo = CST_DTYPE_E4M3, H
     with _on(dev):

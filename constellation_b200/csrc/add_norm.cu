@@ -41,12 +41,14 @@ struct AddNormArgs {
 
 constexpr int kMaxNormWidth = 32768;  // 1024 threads x 32 elements in registers
 
-// A row is held by `warps_per_row` warps, V vectors of VEC elements a thread; a block holds
-// blockDim / 32 / warps_per_row rows.
-template <int VEC, int V>
-__global__ void __launch_bounds__(1024) add_norm_kernel(AddNormArgs a) {
+// A row is held by `warps_per_row` warps, V vectors of 8 elements a thread; a block holds
+// blockDim / 32 / warps_per_row rows.  DT: the type of x, residual, sum and a 16- or 32-bit out when they
+// all have it, 0 otherwise.  F8: the e4m3 form.  ANY: rows that start anywhere; the vectors then begin
+// up to 7 columns before the row, on the 16-byte boundaries of the tensor that is written.
+template <int V, int THREADS, int DT, bool F8, bool ANY>
+__global__ void __launch_bounds__(THREADS) add_norm_kernel(AddNormArgs a) {
     __shared__ float s_part[32];
-    __shared__ float s_max[VEC == 1 ? 32 * V : 1];  // VEC 1: maxima of 32 consecutive elements
+    __shared__ int s_most[F8 && ANY ? kMaxNormWidth / 128 : 1];  // ANY: a row's block maxima, as bits (one row a block)
     chain_wait();
     chain_release();
     const int W = a.warps_per_row, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -54,36 +56,63 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(AddNormArgs a) {
     const int64_t row = int64_t(blockIdx.x) * (int(blockDim.x >> 5) / W) + local;
     const bool live = row < a.T;
     const int tid = threadIdx.x - first_warp * 32, step = W * 32;
-
-    float h[V][VEC];
-    float ss = 0.0f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int c = (tid + v * step) * VEC;
-        const bool in = live && c < a.H;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) h[v][k] = 0.0f;
-        if (in) load_act<VEC>(a.x, a.x_dtype, row * a.ld_x + c, h[v]);
-    }
-    if (a.res) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int c = (tid + v * step) * VEC;
-            if (!(live && c < a.H)) continue;
-            float r[VEC];
-            load_act<VEC>(a.res, a.res_dtype, row * a.ld_res + c, r);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) h[v][k] += r[k];
-            if (a.sum) store_act<VEC>(a.sum, a.res_dtype, row * a.ld_sum + c, h[v]);
+    const int xt = DT ? DT : a.x_dtype, rt = DT ? DT : a.res_dtype, ot = DT ? DT : a.out_dtype;
+    int lead = 0;
+    if constexpr (ANY) {
+        if (live) {
+            lead = a.sum ? lead_in(a.sum, rt, row * a.ld_sum)
+                   : F8  ? int((reinterpret_cast<uintptr_t>(a.out) + row * a.ld_out) & 7u)
+                         : lead_in(a.out, ot, row * a.ld_out);
+        }
+        if constexpr (F8) {
+            for (int i = threadIdx.x; i < (a.H + 127) / 128; i += blockDim.x) s_most[i] = 0;
         }
     }
+    auto column = [&](int v) { return (tid + v * step) * 8 - lead; };
+    // a vector may lie outside the row altogether: beyond its end
+    auto within = [&](int c) { return live && c < a.H; };
+
+    float h[V][8];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int c = column(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[v][k] = 0.0f;
+        if (!within(c)) continue;
+        if constexpr (ANY) load8_any(a.x, xt, row * a.ld_x, c, a.H, h[v]);
+        else load8(a.x, xt, row * a.ld_x + c, h[v]);
+    }
+    if (a.res) {
+        // all loads before the first store, which the compiler has to take for one into the residual
+        float r[V][8];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int c = column(v);
+            if (!within(c)) continue;
+            if constexpr (ANY) load8_any(a.res, rt, row * a.ld_res, c, a.H, r[v]);
+            else load8(a.res, rt, row * a.ld_res + c, r[v]);
+        }
+        // in place, a neighbour's wide read must not meet a store of this row
+        if constexpr (ANY) __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int c = column(v);
+            if (!within(c)) continue;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h[v][k] += r[v][k];
+            if (!a.sum) continue;
+            if constexpr (ANY) store8_any(a.sum, rt, row * a.ld_sum, c, a.H, h[v]);
+            else store8(a.sum, rt, row * a.ld_sum + c, h[v]);
+        }
+    }
+    float ss = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) ss = fmaf(h[v][k], h[v][k], ss);
+        for (int k = 0; k < 8; ++k) ss = fmaf(h[v][k], h[v][k], ss);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (W > 1) {
+    if (W > 1 || ANY) {
         if (lane == 0) s_part[warp] = ss;
         __syncthreads();
         ss = 0.0f;
@@ -92,71 +121,108 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(AddNormArgs a) {
     const float r = rsqrtf(ss / float(a.H) + a.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (tid + v * step) * VEC;
-        if (c >= a.H) continue;
+        const int c = column(v);
+        float w[8];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) h[v][k] = h[v][k] * r * (a.weight ? __ldg(a.weight + c + k) : 1.0f);
-    }
-    if (a.out_dtype != 4) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int c = (tid + v * step) * VEC;
-            if (live && c < a.H) store_act<VEC>(a.out, a.out_dtype, row * a.ld_out + c, h[v]);
+        for (int k = 0; k < 8; ++k) w[k] = 1.0f;
+        if (a.weight && c < a.H) {
+            if constexpr (ANY) load8_any(a.weight, CST_DTYPE_FP32, 0, c, a.H, w);
+            else load8(a.weight, CST_DTYPE_FP32, c, w);
         }
-        return;
-    }
-    // e4m3: the maximum of each 128 columns, 16 threads (VEC 8) or 4 warps' steps (VEC 1)
-    float most[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        most[v] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) most[v] = fmaxf(most[v], fabsf(h[v][k]));
-#pragma unroll
-        for (int o = VEC == 8 ? 8 : 16; o > 0; o >>= 1)
-            most[v] = fmaxf(most[v], __shfl_xor_sync(0xffffffffu, most[v], o));
-    }
-    if constexpr (VEC == 1) {
-        // 32-column piece j of the row at s_max[first_warp * V + j]
-        if (lane == 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) s_max[first_warp * V + v * W + (warp - first_warp)] = most[v];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = v * W + (warp - first_warp), j0 = j & ~3;
-            for (int i = j0; i < j0 + 4 && i < W * V; ++i) most[v] = fmaxf(most[v], s_max[first_warp * V + i]);
+        for (int k = 0; k < 8; ++k) h[v][k] = h[v][k] * r * w[k];
+        if constexpr (!F8) {
+            if (!within(c)) continue;
+            if constexpr (ANY) store8_any(a.out, ot, row * a.ld_out, c, a.H, h[v]);
+            else store8(a.out, ot, row * a.ld_out + c, h[v]);
         }
     }
-    const int blocks = (a.H + 127) / 128;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int c = (tid + v * step) * VEC;
-        if (!live || c >= a.H) continue;
+    if constexpr (F8) {
         // a block of zeros takes scale 1; the smallest normal keeps 1 / s finite
-        const float s = most[v] == 0.0f ? 1.0f : fmaxf(most[v] / 448.0f, FLT_MIN);
-        const float inv = 1.0f / s;
-        if (c % 128 == 0) a.scale[row * blocks + c / 128] = s;
-        uint8_t* o = static_cast<uint8_t*>(a.out) + row * a.ld_out + c;
-        if constexpr (VEC == 1) {
-            *o = e4m3_rn(h[v][0] * inv);
-        } else {
-            uint32_t q[4];
+        auto scale_of = [](float most) { return most == 0.0f ? 1.0f : fmaxf(most / 448.0f, FLT_MIN); };
+        const int blocks = (a.H + 127) / 128;
+        uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.ld_out;
+        if constexpr (!ANY) {
+            // the maximum of 128 columns: 16 threads
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q[k] = e4m3x2_rn(h[v][2 * k] * inv, h[v][2 * k + 1] * inv);
-            *reinterpret_cast<uint2*>(o) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+            for (int v = 0; v < V; ++v) {
+                const int c = column(v);
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(h[v][k]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (!within(c)) continue;
+                const float s = scale_of(most), inv = 1.0f / s;
+                if (c % 128 == 0) a.scale[row * blocks + c / 128] = s;
+                uint32_t q[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = e4m3x2_rn(h[v][2 * k] * inv, h[v][2 * k + 1] * inv);
+                *reinterpret_cast<uint2*>(out + c) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+            }
+        } else {
+            // a vector may belong to two blocks; the maximum does not depend on the order it is taken in
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int c = column(v);
+                if (!within(c)) continue;
+                const int b0 = max(c, 0) >> 7, edge = (b0 + 1) << 7;
+                float most0 = 0.0f, most1 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {  // columns outside the row are zero
+                    const float m = fabsf(h[v][k]);
+                    most0 = fmaxf(most0, c + k < edge ? m : 0.0f);
+                    most1 = fmaxf(most1, c + k < edge ? 0.0f : m);
+                }
+                atomicMax(&s_most[b0], __float_as_int(most0));
+                if (c + 8 > edge && edge < a.H) atomicMax(&s_most[b0 + 1], __float_as_int(most1));
+            }
+            __syncthreads();
+            if (live)
+                for (int i = tid; i < blocks; i += step) a.scale[row * blocks + i] = scale_of(__int_as_float(s_most[i]));
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int c = column(v);
+                if (!within(c)) continue;
+                const int b0 = max(c, 0) >> 7, edge = (b0 + 1) << 7;
+                const float inv0 = 1.0f / scale_of(__int_as_float(s_most[b0]));
+                const float inv1 = c + 8 > edge && edge < a.H ? 1.0f / scale_of(__int_as_float(s_most[b0 + 1])) : inv0;
+                uint32_t q[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    q[k] = e4m3x2_rn(h[v][2 * k] * (c + 2 * k >= edge ? inv1 : inv0),
+                                     h[v][2 * k + 1] * (c + 2 * k + 1 >= edge ? inv1 : inv0));
+                const uint2 both = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+                if (c >= 0 && c + 8 <= a.H && (reinterpret_cast<uintptr_t>(out + c) & 7u) == 0) {
+                    *reinterpret_cast<uint2*>(out + c) = both;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (unsigned(c + k) < unsigned(a.H))
+                            out[c + k] = uint8_t((k < 4 ? both.x >> (8 * k) : both.y >> (8 * (k - 4))) & 255u);
+                }
+            }
         }
     }
 }
 
-template <int VEC, int V>
+template <int V, int THREADS, int DT, bool ANY>
 cudaError_t launch(AddNormArgs a, cudaStream_t stream) {
-    int W = 1;
-    while (W * 32 * V * VEC < a.H) W *= 2;
+    const int W = (a.H + (ANY ? 7 : 0) + 32 * V * 8 - 1) / (32 * V * 8);  // ANY: up to 7 columns before the row
     a.warps_per_row = W;
-    const int warps = W < 8 ? 8 : W, rows = warps / W;
-    return launch_chained(add_norm_kernel<VEC, V>, dim3((a.T + rows - 1) / rows), dim3(warps * 32), 0, stream, a);
+    const int rows = ANY || W >= 8 ? 1 : 8 / W;
+    auto kernel = a.out_dtype == CST_DTYPE_E4M3 ? add_norm_kernel<V, THREADS, DT, true, ANY>
+                                                : add_norm_kernel<V, THREADS, DT, false, ANY>;
+    return launch_chained(kernel, dim3((a.T + rows - 1) / rows), dim3(rows * W * 32), 0, stream, a);
+}
+
+template <int DT>
+cudaError_t launch_aligned(const AddNormArgs& a, cudaStream_t s) {
+    // Few rows: as many threads a row as it has vectors.  Many: 4 vectors a thread, whose loads are all in
+    // flight at once.
+    return a.H > 8192 ? launch<4, 1024, DT, false>(a, s)
+           : a.T <= 592 ? launch<1, 1024, DT, false>(a, s)
+                        : launch<4, 256, DT, false>(a, s);
 }
 
 }  // namespace
@@ -185,14 +251,20 @@ extern "C" int cst_add_rmsnorm(const void* x, int32_t x_dtype, int64_t ld_x, con
         return set_last_error(CST_ERR_INVALID_ARG, "null x, out or scale");
     AddNormArgs a{x, x_dtype, ld_x, residual, residual_dtype, ld_residual, T, H, weight, eps, sum, ld_sum, out,
                   out_dtype, ld_out, scale, 0};
-    const bool vec = H % 8 == 0 && rows_aligned16(x, ld_x, act_size(x_dtype)) &&
-                     (!residual || rows_aligned16(residual, ld_residual, act_size(residual_dtype))) &&
-                     (!sum || rows_aligned16(sum, ld_sum, act_size(residual_dtype))) &&
-                     (out_dtype == CST_DTYPE_E4M3
-                          ? (reinterpret_cast<uintptr_t>(out) % 8 == 0 && ld_out % 8 == 0)
-                          : rows_aligned16(out, ld_out, act_size(out_dtype)));
+    const bool f8 = out_dtype == CST_DTYPE_E4M3;
+    const bool aligned = H % 8 == 0 && (reinterpret_cast<uintptr_t>(weight) & 15u) == 0 &&
+                         rows_aligned16(x, ld_x, act_size(x_dtype)) &&
+                         (!residual || rows_aligned16(residual, ld_residual, act_size(residual_dtype))) &&
+                         (!sum || rows_aligned16(sum, ld_sum, act_size(residual_dtype))) &&
+                         (f8 ? (reinterpret_cast<uintptr_t>(out) % 8 == 0 && ld_out % 8 == 0)
+                             : rows_aligned16(out, ld_out, act_size(out_dtype)));
+    const bool same = (!residual || residual_dtype == x_dtype) && (f8 || out_dtype == x_dtype);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = vec ? launch<8, 4>(a, s) : launch<1, 32>(a, s);
+    const cudaError_t e = !aligned ? (H <= 8185 ? launch<1, 1024, 0, true>(a, s) : launch<5, 1024, 0, true>(a, s))
+                          : !same  ? launch_aligned<0>(a, s)
+                          : x_dtype == CST_DTYPE_BF16 ? launch_aligned<2>(a, s)
+                          : x_dtype == CST_DTYPE_FP16 ? launch_aligned<1>(a, s)
+                                                      : launch_aligned<3>(a, s);
     if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "add_rmsnorm launch failed: %s", cudaGetErrorString(e));
     return CST_OK;
 }

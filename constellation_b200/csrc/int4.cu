@@ -146,14 +146,10 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
     const bool vec = (reinterpret_cast<uintptr_t>(x) + at * 2) % 16 == 0;
     auto load = [&](int c, float (&v)[8]) {
         if (vec) {
-            load_act<8>(x, x_dtype, at + c, v);
+            load8(x, x_dtype, at + c, v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float e[1];
-                load_act<1>(x, x_dtype, at + c + j, e);
-                v[j] = e[0];
-            }
+            for (int j = 0; j < 8; ++j) v[j] = load1(x, x_dtype, at + c + j);
         }
         // e4m3 has no infinities: one makes its row's results NaN, as a NaN does
 #pragma unroll
@@ -714,9 +710,8 @@ __device__ __forceinline__ void write_out(const Int4Args& a, const Item& it, int
         y *= gate / (1.0f + expf(-gate));
         col >>= 1;
     }
-    const float v[1] = {y};
     if (col < a.g.out_n && !(a.g.swiglu && (row & 1)))
-        store_act<1>(a.out, a.out_dtype, int64_t(it.row + t) * a.ld_out + col, v);
+        store1(a.out, a.out_dtype, int64_t(it.row + t) * a.ld_out + col, y);
 }
 
 __device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kSets * 128) : "memory"); }
@@ -844,9 +839,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
         const int used = sh.row[g.E], lead = sh.row[0];
         const int64_t outside = int64_t(lead) + (a.R - used);
         for (int64_t r = blockIdx.x; r < outside; r += gridDim.x) {
-            const float zero[1] = {0.0f};
             for (int n = int(threadIdx.x) - kWarpOut * 32; n < g.out_n; n += kSets * 128)
-                store_act<1>(a.out, a.out_dtype, (r < lead ? r : r - lead + used) * a.ld_out + n, zero);
+                store1(a.out, a.out_dtype, (r < lead ? r : r - lead + used) * a.ld_out + n, 0.0f);
         }
         out_role<TERMS, GROUPS>(a, sh, s_part, sp, rank);
     }

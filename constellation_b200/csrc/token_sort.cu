@@ -27,9 +27,11 @@ namespace {
 // ---- order ------------------------------------------------------------------------------
 // A stable counting sort by one cluster: every warp owns a contiguous run of routes and a
 // histogram of its own in shared memory; the CTAs read one another's totals over distributed
-// shared memory, so there is one launch and no workspace.
+// shared memory, so there is one launch and no workspace.  A run is taken 256 routes at a time, whose
+// loads are all in flight at once: the wait for memory, not the counting, is what a run costs.
 
-constexpr int kSortWarps = 16;
+constexpr int kSortWarps = 32;
+constexpr int kSortHeld = 8;  // routes of a lane at a time
 constexpr int kSortMaxCluster = 8;
 constexpr int kSortMaxExperts = 1024;
 
@@ -67,12 +69,24 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
     const int per = (a.n + runs - 1) / runs;
     const int lo = int(min(int64_t(run) * per, int64_t(a.n))), hi = int(min(int64_t(lo) + per, int64_t(a.n)));
     int32_t* mine = s_hist + warp * B;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < hi ? local_expert(a, i) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-        __syncwarp();
+    int held[kSortHeld];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j) {
+            const int i = i0 + j * 32 + lane;
+            held[j] = i < hi ? local_expert(a, i) : -1;
+        }
+    };
+    for (int i0 = lo; i0 < hi; i0 += 32 * kSortHeld) {
+        load(i0);
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j) {
+            if (i0 + j * 32 >= hi) break;
+            const int e = held[j];
+            const unsigned peers = __match_any_sync(0xffffffffu, e);
+            if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
+            __syncwarp();
+        }
     }
     __syncthreads();
     // per expert: exclusive prefix over the warps, and this CTA's total
@@ -117,18 +131,22 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
         __syncthreads();
     }
     cluster.sync();  // no CTA leaves while another still reads its totals
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < hi ? local_expert(a, i) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0) {
-            const int row = s_base[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
-            a.row_of[i] = e == a.E ? -1 : row;
-            a.route_of[row] = e == a.E ? -1 : i;
+    for (int i0 = lo; i0 < hi; i0 += 32 * kSortHeld) {
+        if (hi - lo > 32 * kSortHeld) load(i0);  // a short run is still held
+#pragma unroll
+        for (int j = 0; j < kSortHeld; ++j) {
+            if (i0 + j * 32 >= hi) break;
+            const int i = i0 + j * 32 + lane, e = held[j];
+            const unsigned peers = __match_any_sync(0xffffffffu, e);
+            if (e >= 0) {
+                const int row = s_base[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
+                a.row_of[i] = e == a.E ? -1 : row;
+                a.route_of[row] = e == a.E ? -1 : i;
+            }
+            __syncwarp();
+            if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
+            __syncwarp();
         }
-        __syncwarp();
-        if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-        __syncwarp();
     }
 }
 
@@ -137,51 +155,89 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
 struct CopyArgs {
     const uint8_t* x;  // [T] rows of `bytes`, ld_x bytes apart
     int64_t bytes, ld_x;
-    const uint8_t* scale;  // second plane (row scales), or null
-    int64_t sbytes, ld_scale;
+    const uint32_t* scale;  // [T] rows of n_scale words, ld_scale words apart, or null
+    int n_scale;
+    int64_t ld_scale;
     int T, K;
     const int32_t* row_of;
     const int32_t* rows_used;
-    uint8_t* rows;   // [T * K] rows of `bytes`, packed
-    uint8_t* srows;  // [T * K] rows of `sbytes`, packed
+    uint8_t* rows;    // [T * K] rows of `bytes`, packed
+    uint32_t* srows;  // [T * K] rows of n_scale words, packed
 };
 
-template <typename U>
-__device__ __forceinline__ void spread(const uint8_t* src, uint8_t* rows, int64_t bytes, const int32_t* row, int K,
-                                       int R) {
-    const U* s = reinterpret_cast<const U*>(src);
-    const int64_t n = bytes / int64_t(sizeof(U));
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const U v = s[i];
-        for (int k = 0; k < K; ++k) {
-            const int r = __ldg(row + k);
-            if (unsigned(r) < unsigned(R)) reinterpret_cast<U*>(rows + r * bytes)[i] = v;
-        }
+// Bytes [at, at + 16) of a row of `bytes`, of which those in the row are written; dst + at is 16-byte aligned.
+__device__ __forceinline__ void store16_any(uint8_t* dst, int64_t at, int64_t bytes, const uint4& u) {
+    if (at >= 0 && at + 16 <= bytes) {
+        *reinterpret_cast<uint4*>(dst + at) = u;
+    } else {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (uint64_t(at + k) < uint64_t(bytes)) dst[at + k] = uint8_t(w[k >> 2] >> (8 * (k & 3)));
     }
 }
 
-template <typename U>
-__device__ __forceinline__ void clear(uint8_t* dst, int64_t bytes) {
-    const int64_t n = bytes / int64_t(sizeof(U));
-    U z{};
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<U*>(dst)[i] = z;
+// ANY: rows that start anywhere.  Each copy of a row then lies on 16-byte boundaries of its own, and its
+// pieces are read shifted from the one source row, which the CTA's first copy brought into L1.
+template <bool ANY>
+__device__ __forceinline__ void copy_row(const uint8_t* src, uint8_t* dst, int64_t bytes) {
+    const int64_t lead = ANY ? int64_t(reinterpret_cast<uintptr_t>(dst) & 15u) : 0;
+    for (int64_t at = int64_t(threadIdx.x) * 16 - lead; at < bytes; at += int64_t(blockDim.x) * 16) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (src == nullptr) {
+        } else if (!ANY) {
+            u = *reinterpret_cast<const uint4*>(src + at);
+        } else if (at >= 16 && at + 32 <= bytes) {
+            u = load16_any(src + at);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (uint64_t(at + k) < uint64_t(bytes)) w[k >> 2] |= uint32_t(src[at + k]) << (8 * (k & 3));
+            u = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (!ANY) *reinterpret_cast<uint4*>(dst + at) = u;
+        else store16_any(dst, at, bytes, u);
+    }
 }
 
-// Blocks of tokens first, then the rows behind the last expert's.
-template <typename U, typename S>
+// Blocks of tokens; each also clears its share of the rows behind the last expert's.
+template <bool ANY>
 __global__ void __launch_bounds__(256) sort_rows_kernel(CopyArgs a) {
     chain_wait();
     chain_release();
     const int R = a.T * a.K;
     for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
         const int32_t* row = a.row_of + int64_t(t) * a.K;
-        spread<U>(a.x + t * a.ld_x, a.rows, a.bytes, row, a.K, R);
-        if (a.scale) spread<S>(a.scale + t * a.ld_scale, a.srows, a.sbytes, row, a.K, R);
+        const uint8_t* src = a.x + t * a.ld_x;
+        if (a.scale) {
+            for (int i = threadIdx.x; i < a.n_scale * a.K; i += blockDim.x) {
+                const int k = i / a.n_scale, c = i - k * a.n_scale, r = __ldg(row + k);
+                if (unsigned(r) < unsigned(R)) a.srows[int64_t(r) * a.n_scale + c] = a.scale[t * a.ld_scale + c];
+            }
+        }
+        if constexpr (ANY) {
+            for (int k = 0; k < a.K; ++k) {
+                const int r = __ldg(row + k);
+                if (unsigned(r) < unsigned(R)) copy_row<true>(src, a.rows + r * a.bytes, a.bytes);
+            }
+        } else {
+            // each piece is read once and stored K times
+            for (int64_t at = int64_t(threadIdx.x) * 16; at < a.bytes; at += int64_t(blockDim.x) * 16) {
+                const uint4 u = *reinterpret_cast<const uint4*>(src + at);
+#pragma unroll 4
+                for (int k = 0; k < a.K; ++k) {
+                    const int r = __ldg(row + k);
+                    if (unsigned(r) < unsigned(R)) *reinterpret_cast<uint4*>(a.rows + r * a.bytes + at) = u;
+                }
+            }
+        }
     }
     const int used = max(0, min(*a.rows_used, R));
     for (int64_t r = used + int64_t(blockIdx.x); r < R; r += gridDim.x) {
-        clear<U>(a.rows + r * a.bytes, a.bytes);
-        if (a.scale) clear<S>(a.srows + r * a.sbytes, a.sbytes);
+        copy_row<ANY>(nullptr, a.rows + r * a.bytes, a.bytes);
+        if (a.scale)
+            for (int c = threadIdx.x; c < a.n_scale; c += blockDim.x) a.srows[r * a.n_scale + c] = 0u;
     }
 }
 
@@ -201,33 +257,68 @@ struct UnsortArgs {
     int out_dtype;
 };
 
-template <int VEC>
-__global__ void __launch_bounds__(256) unsort_kernel(UnsortArgs a) {
+// A thread takes 8 columns of a token and loads them of up to 8 of its rows before it adds any, so a sum costs
+// one wait for memory.  DT: the rows' type where it is 16 bits, 0 otherwise.  Vectors are numbered through
+// all tokens, so that narrow rows fill a CTA.
+template <int DT, bool ANY>
+__global__ void __launch_bounds__(256) unsort_kernel(UnsortArgs a, int vectors) {
+    constexpr int kAhead = 8;
     chain_wait();
     chain_release();
-    const int t = blockIdx.x, R = a.T * a.K;
-    const int32_t* row = a.row_of + int64_t(t) * a.K;
-    const float* weight = a.weight ? a.weight + int64_t(t) * a.K : nullptr;
-    for (int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC; c < a.H; c += gridDim.y * blockDim.x * VEC) {
-        float acc[VEC];
+    const int R = a.T * a.K;
+    const int64_t all = int64_t(a.T) * vectors;
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += int64_t(gridDim.x) * blockDim.x) {
+        const int t = int(i / vectors), at = int(i - int64_t(t) * vectors) * 8;
+        const int64_t out_row = int64_t(t) * a.H;
+        const int c = ANY ? at - lead_in(a.out, a.out_dtype, out_row) : at;
+        if (ANY && c >= a.H) continue;
+        const int32_t* row = a.row_of + int64_t(t) * a.K;
+        const float* weight = a.weight ? a.weight + int64_t(t) * a.K : nullptr;
+        float acc[8];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-        for (int k = 0; k < a.K; ++k) {
-            const int r = __ldg(row + k);
-            if (unsigned(r) >= unsigned(R)) continue;
-            const float w = weight ? __ldg(weight + k) : 1.0f;
-            float v[VEC];
-            load_act<VEC>(a.rows, a.dtype, r * a.ld + c, v);
+        for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+        for (int k0 = 0; k0 < a.K; k0 += kAhead) {
+            if constexpr (DT != 0 && !ANY) {
+                uint4 u[kAhead];
+                float w[kAhead];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+                for (int k = 0; k < kAhead; ++k) {
+                    const int r = k0 + k < a.K ? __ldg(row + k0 + k) : -1;
+                    const bool here = unsigned(r) < unsigned(R);
+                    u[k] = here ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.rows) + r * a.ld + c)
+                                : make_uint4(0, 0, 0, 0);
+                    w[k] = !here ? 0.0f : weight ? __ldg(weight + k0 + k) : 1.0f;  // an absent route's weight is not used
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    float v[8];
+                    unpack8(u[k], DT, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[k], v[j], acc[j]);
+                }
+            } else {
+#pragma unroll 4
+                for (int k = k0; k < min(k0 + kAhead, a.K); ++k) {
+                    const int r = __ldg(row + k);
+                    if (unsigned(r) >= unsigned(R)) continue;
+                    const float w = weight ? __ldg(weight + k) : 1.0f;
+                    float v[8];
+                    if constexpr (ANY) load8_any(a.rows, a.dtype, r * a.ld, c, a.H, v);
+                    else load8(a.rows, a.dtype, r * a.ld + c, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, v[j], acc[j]);
+                }
+            }
         }
         if (a.res) {
-            float v[VEC];
-            load_act<VEC>(a.res, a.res_dtype, t * a.ld_res + c, v);
+            float v[8];
+            if constexpr (ANY) load8_any(a.res, a.res_dtype, t * a.ld_res, c, a.H, v);
+            else load8(a.res, a.res_dtype, t * a.ld_res + c, v);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+            for (int j = 0; j < 8; ++j) acc[j] += v[j];
         }
-        store_act<VEC>(a.out, a.out_dtype, int64_t(t) * a.H + c, acc);
+        if constexpr (ANY) store8_any(a.out, a.out_dtype, out_row, c, a.H, acc);
+        else store8(a.out, a.out_dtype, out_row + c, acc);
     }
 }
 
@@ -246,63 +337,129 @@ struct UnsortGradArgs {
     float* d_weight;  // [T, K], or null
 };
 
-template <int VEC>
+// One CTA a token, kAhead of its routes at a time: a thread loads 8 columns of the gradient and of these routes'
+// rows together, stores the rows' gradients and keeps a partial dot product for each.  DT: the type of g, rows and
+// d_rows where all have it, 0 otherwise.
+template <int DT, bool ANY>
 __global__ void __launch_bounds__(256) unsort_grad_kernel(UnsortGradArgs a) {
-    __shared__ float s_part[8];
+    constexpr int kAhead = 8;
+    __shared__ float s_part[8][kAhead];
     chain_wait();
     chain_release();
-    const int R = a.T * a.K;
+    const int R = a.T * a.K, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gt = DT ? DT : a.g_dtype, dt = DT ? DT : a.dtype;
     for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
-        for (int k = 0; k < a.K; ++k) {
-            const int r = __ldg(a.row_of + int64_t(t) * a.K + k);
-            const bool here = unsigned(r) < unsigned(R);
-            const float w = a.weight ? __ldg(a.weight + int64_t(t) * a.K + k) : 1.0f;
-            float dot = 0.0f;
-            if (here) {
-                for (int c = threadIdx.x * VEC; c < a.H; c += blockDim.x * VEC) {
-                    float g[VEC], v[VEC];
-                    load_act<VEC>(a.g, a.g_dtype, t * a.ld_g + c, g);
-                    if (a.d_weight) {
-                        load_act<VEC>(a.rows, a.dtype, r * a.ld + c, v);
+        for (int k0 = 0; k0 < a.K; k0 += kAhead) {
+            int r[kAhead];
+            float w[kAhead], dot[kAhead];
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) dot = fmaf(g[i], v[i], dot);
+            for (int k = 0; k < kAhead; ++k) {
+                const int at = k0 + k < a.K ? __ldg(a.row_of + int64_t(t) * a.K + k0 + k) : -1;
+                r[k] = unsigned(at) < unsigned(R) ? at : -1;
+                w[k] = r[k] >= 0 && a.weight ? __ldg(a.weight + int64_t(t) * a.K + k0 + k) : 1.0f;
+                dot[k] = 0.0f;
+            }
+            if constexpr (!ANY) {
+                for (int c = threadIdx.x * 8; c < a.H; c += blockDim.x * 8) {
+                    float g[8];
+                    load8(a.g, gt, t * a.ld_g + c, g);
+                    if constexpr (DT == 1 || DT == 2) {
+                        uint4 u[kAhead];
+                        if (a.d_weight) {
+#pragma unroll
+                            for (int k = 0; k < kAhead; ++k)
+                                if (r[k] >= 0)
+                                    u[k] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.rows) + r[k] * a.ld + c);
+                        }
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k) {
+                            if (r[k] < 0) continue;
+                            float v[8];
+                            if (a.d_weight) {
+                                unpack8(u[k], DT, v);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) dot[k] = fmaf(g[j], v[j], dot[k]);
+                            }
+                            if (a.d_rows) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] = w[k] * g[j];
+                                store8(a.d_rows, DT, int64_t(r[k]) * a.H + c, v);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k) {
+                            if (r[k] < 0) continue;
+                            float v[8];
+                            if (a.d_weight) {
+                                load8(a.rows, dt, r[k] * a.ld + c, v);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) dot[k] = fmaf(g[j], v[j], dot[k]);
+                            }
+                            if (a.d_rows) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] = w[k] * g[j];
+                                store8(a.d_rows, dt, int64_t(r[k]) * a.H + c, v);
+                            }
+                        }
                     }
-                    if (a.d_rows) {
+                }
+            } else {
+                // each route's vectors lie on the 16-byte boundaries of the row that is written
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) v[i] = w * g[i];
-                        store_act<VEC>(a.d_rows, a.dtype, int64_t(r) * a.H + c, v);
+                for (int k = 0; k < kAhead; ++k) {
+                    if (r[k] < 0) continue;
+                    const int64_t d_row = int64_t(r[k]) * a.H;
+                    const int lead = a.d_rows ? lead_in(a.d_rows, dt, d_row) : 0;
+                    for (int c = threadIdx.x * 8 - lead; c < a.H; c += blockDim.x * 8) {
+                        float g[8], v[8];
+                        load8_any(a.g, gt, t * a.ld_g, c, a.H, g);
+                        if (a.d_weight) {
+                            load8_any(a.rows, dt, r[k] * a.ld, c, a.H, v);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (unsigned(c + j) < unsigned(a.H)) dot[k] = fmaf(g[j], v[j], dot[k]);
+                        }
+                        if (a.d_rows) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = w[k] * g[j];
+                            store8_any(a.d_rows, dt, d_row, c, a.H, v);
+                        }
                     }
                 }
             }
-            if (a.d_weight) {
+            if (!a.d_weight) continue;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = dot;
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    float sum = 0.0f;
-                    for (int i = 0; i < 8; ++i) sum += s_part[i];
-                    a.d_weight[int64_t(t) * a.K + k] = here ? sum : 0.0f;
-                }
-                __syncthreads();
+            for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+                if (lane == 0) s_part[warp][k] = dot[k];
             }
+            __syncthreads();
+            if (threadIdx.x < kAhead && k0 + int(threadIdx.x) < a.K) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += s_part[i][threadIdx.x];
+                a.d_weight[int64_t(t) * a.K + k0 + threadIdx.x] = sum;  // 0 for an absent route
+            }
+            __syncthreads();
         }
     }
     if (!a.d_rows) return;
     const int used = max(0, min(*a.rows_used, R));
-    float zero[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero[i] = 0.0f;
+    const int64_t bytes = int64_t(a.H) * (dt == 3 ? 4 : 2);
     for (int64_t r = used + int64_t(blockIdx.x); r < R; r += gridDim.x)
-        for (int c = threadIdx.x * VEC; c < a.H; c += blockDim.x * VEC)
-            store_act<VEC>(a.d_rows, a.dtype, r * a.H + c, zero);
+        copy_row<ANY>(nullptr, static_cast<uint8_t*>(a.d_rows) + r * bytes, bytes);
 }
 
 cudaError_t launch_order(const OrderArgs& a, cudaStream_t stream) {
     const size_t smem = size_t(kSortWarps + 2) * (a.E + 1) * 4;
-    cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-    const int ranks = a.n > 4096 ? kSortMaxCluster : 1;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) return e;
+    }
+    // one CTA counts 256 routes a warp without reading them twice; beyond that the cluster shares them
+    const int ranks = a.n > kSortWarps * 32 * kSortHeld / 2 ? kSortMaxCluster : 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ranks);
     cfg.blockDim = dim3(kSortWarps * 32);
@@ -320,19 +477,6 @@ cudaError_t launch_order(const OrderArgs& a, cudaStream_t stream) {
 }
 
 bool act_dtype(int d) { return d >= CST_DTYPE_FP16 && d <= CST_DTYPE_FP32; }
-
-// The largest power of two up to 16 that divides all of a plane's addresses and strides.
-int copy_unit(const void* a, const void* b, int64_t bytes, int64_t ld) {
-    const uint64_t all = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | uint64_t(bytes) |
-                         uint64_t(ld) | 16u;
-    return int(all & (~all + 1));
-}
-
-template <typename U>
-cudaError_t launch_sort_rows(const CopyArgs& a, int sunit, int grid, cudaStream_t s) {
-    if (sunit >= 16) return launch_chained(sort_rows_kernel<U, uint4>, dim3(grid), dim3(256), 0, s, a);
-    return launch_chained(sort_rows_kernel<U, uint32_t>, dim3(grid), dim3(256), 0, s, a);
-}
 
 int check_routes(const char* what, int64_t T, int64_t K) {
     if (T < 0 || K < 1 || K > CST_SORT_MAX_TOP_K || T * K > (int64_t(1) << 30))
@@ -378,21 +522,16 @@ extern "C" int cst_sort_rows(const void* x, int64_t row_bytes, int64_t ld_bytes,
     if (T == 0) return CST_OK;
     if (!x || !row_of || !rows_used || !rows || (scale && !rows_scale))
         return set_last_error(CST_ERR_INVALID_ARG, "null x, order or rows");
-    const CopyArgs a{static_cast<const uint8_t*>(x), row_bytes, ld_bytes, reinterpret_cast<const uint8_t*>(scale),
-                     int64_t(n_scale) * 4, ld_scale * 4, T, K, row_of, rows_used, static_cast<uint8_t*>(rows),
-                     reinterpret_cast<uint8_t*>(rows_scale)};
+    const CopyArgs a{static_cast<const uint8_t*>(x), row_bytes, ld_bytes, reinterpret_cast<const uint32_t*>(scale),
+                     n_scale, ld_scale, T, K, row_of, rows_used, static_cast<uint8_t*>(rows),
+                     reinterpret_cast<uint32_t*>(rows_scale)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int unit = copy_unit(x, rows, row_bytes, ld_bytes);
-    const int sunit = scale ? copy_unit(scale, rows_scale, a.sbytes, a.ld_scale) : 4;
-    const int grid = T;
-    cudaError_t e;
-    switch (unit) {
-        case 16: e = launch_sort_rows<uint4>(a, sunit, grid, s); break;
-        case 8: e = launch_sort_rows<uint2>(a, sunit, grid, s); break;
-        case 4: e = launch_sort_rows<uint32_t>(a, sunit, grid, s); break;
-        case 2: e = launch_sort_rows<uint16_t>(a, sunit, grid, s); break;
-        default: e = launch_sort_rows<uint8_t>(a, sunit, grid, s); break;
-    }
+    const bool aligned = row_bytes % 16 == 0 && rows_aligned16(x, ld_bytes, 1) && rows_aligned16(rows, row_bytes, 1);
+    // as many threads as a row has pieces, up to 256
+    const int64_t pieces = (row_bytes + 15) / 16;
+    const int threads = pieces >= 256 ? 256 : int((pieces + 31) / 32 * 32);
+    const cudaError_t e = launch_chained(aligned ? sort_rows_kernel<false> : sort_rows_kernel<true>, dim3(T), dim3(threads),
+                                         0, s, a);
     return launched("sort_rows", e);
 }
 
@@ -415,10 +554,14 @@ extern "C" int cst_unsort_rows(const void* rows, int32_t rows_dtype, int64_t ld_
                      rows_aligned16(out, H, act_size(out_dtype)) &&
                      (!residual || rows_aligned16(residual, ld_residual, act_size(residual_dtype)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int V = vec ? 8 : 1;
-    const dim3 grid(T, (H + 256 * V - 1) / (256 * V));
-    return launched("unsort_rows", vec ? launch_chained(unsort_kernel<8>, grid, dim3(256), 0, s, a)
-                                       : launch_chained(unsort_kernel<1>, grid, dim3(256), 0, s, a));
+    const int vectors = (H + 7) / 8 + (vec ? 0 : 1);  // anywhere: up to 7 columns before the row
+    const int64_t ctas = (int64_t(T) * vectors + 255) / 256;
+    auto kernel = !vec ? unsort_kernel<0, true>
+                  : rows_dtype == CST_DTYPE_BF16 ? unsort_kernel<2, false>
+                  : rows_dtype == CST_DTYPE_FP16 ? unsort_kernel<1, false>
+                                                 : unsort_kernel<0, false>;
+    return launched("unsort_rows", launch_chained(kernel, dim3(unsigned(ctas < INT32_MAX ? ctas : INT32_MAX)), dim3(256), 0,
+                                                  s, a, vectors));
 }
 
 extern "C" int cst_unsort_rows_grad(const void* grad, int32_t grad_dtype, int64_t ld_grad, const void* rows,
@@ -440,6 +583,11 @@ extern "C" int cst_unsort_rows_grad(const void* grad, int32_t grad_dtype, int64_
                      (!d_weight || rows_aligned16(rows, ld_rows, act_size(rows_dtype))) &&
                      (!d_rows || rows_aligned16(d_rows, H, act_size(rows_dtype)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return launched("unsort_rows_grad", vec ? launch_chained(unsort_grad_kernel<8>, dim3(T), dim3(256), 0, s, a)
-                                            : launch_chained(unsort_grad_kernel<1>, dim3(T), dim3(256), 0, s, a));
+    const bool same = grad_dtype == rows_dtype;
+    auto kernel = !vec ? unsort_grad_kernel<0, true>
+                  : !same ? unsort_grad_kernel<0, false>
+                  : rows_dtype == CST_DTYPE_BF16 ? unsort_grad_kernel<2, false>
+                  : rows_dtype == CST_DTYPE_FP16 ? unsort_grad_kernel<1, false>
+                                                 : unsort_grad_kernel<3, false>;
+    return launched("unsort_rows_grad", launch_chained(kernel, dim3(T), dim3(256), 0, s, a));
 }
