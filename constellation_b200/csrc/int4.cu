@@ -1081,10 +1081,7 @@ extern "C" int cst_grouped_int4(const cst_int4_weight* w, void* data, const void
         return set_last_error(CST_ERR_INVALID_ARG, "null data, x, workspace or out");
     if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(workspace)) & 15u))
         return set_last_error(CST_ERR_INVALID_ARG, "data and workspace must be 16-byte aligned");
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "cannot query the SM count: %s", cudaGetErrorString(e));
+    const int sms = current_sms();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Int4Args a{};
     a.g = g;

@@ -28,6 +28,15 @@ cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// SMs of the current device (148 where that cannot be asked).
+inline int current_sms() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return sms;
+}
+
 // capi.cu: the thread's cst_last_error() message, for entry points in other files
 void clear_last_error();
 int set_last_error(int code, const char* fmt, ...);
