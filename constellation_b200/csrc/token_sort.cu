@@ -30,7 +30,7 @@ namespace {
 // shared memory, so there is one launch and no workspace.  A run is taken 256 routes at a time, whose
 // loads are all in flight at once: the wait for memory, not the counting, is what a run costs.
 
-constexpr int kSortWarps = 32;
+constexpr int kSortMaxWarps = 32, kSortMinWarps = 8;
 constexpr int kSortHeld = 8;  // routes of a lane at a time
 constexpr int kSortMaxCluster = 8;
 constexpr int kSortMaxExperts = 1024;
@@ -40,6 +40,7 @@ struct OrderArgs {
     int idx64;
     int n;  // routes
     int E, first;
+    int bits;  // of a number up to E, and one more, which only -1 has
     int32_t* row_of;
     int32_t* route_of;
     int32_t* offsets;
@@ -51,21 +52,32 @@ __device__ __forceinline__ int local_expert(const OrderArgs& a, int i) {
     return (v >= 0 && e >= 0 && e < a.E) ? int(e) : a.E;
 }
 
-__global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
-    extern __shared__ int32_t s_hist[];  // [kSortWarps][E + 1], then totals [E + 1], then bases [E + 2]
-    __shared__ int32_t s_warp[kSortWarps];
+// The lanes whose expert is this lane's, from one vote a bit of the expert's number (-1 has all of them set).
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+    unsigned peers = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = (e >> b) & 1;
+        const unsigned vote = __ballot_sync(0xffffffffu, set);
+        peers &= set ? vote : ~vote;
+    }
+    return peers;
+}
+
+__global__ void __launch_bounds__(kSortMaxWarps * 32) order_kernel(OrderArgs a) {
+    extern __shared__ int32_t s_hist[];  // [warps][E + 1], then totals [E + 1], then bases [E + 1]
+    __shared__ int32_t s_warp[kSortMaxWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
-    const int B = a.E + 1;
-    int32_t* s_total = s_hist + kSortWarps * B;
+    const int B = a.E + 1, warps = blockDim.x >> 5;
+    int32_t* s_total = s_hist + warps * B;
     int32_t* s_base = s_total + B;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < kSortWarps * B; i += blockDim.x) s_hist[i] = 0;
+    for (int i = threadIdx.x; i < warps * B; i += blockDim.x) s_hist[i] = 0;
     chain_wait();
     chain_release();
     __syncthreads();
     // this warp's routes [lo, hi)
-    const int runs = ranks * kSortWarps, run = rank * kSortWarps + warp;
+    const int runs = ranks * warps, run = rank * warps + warp;
     const int per = (a.n + runs - 1) / runs;
     const int lo = int(min(int64_t(run) * per, int64_t(a.n))), hi = int(min(int64_t(lo) + per, int64_t(a.n)));
     int32_t* mine = s_hist + warp * B;
@@ -82,17 +94,14 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
 #pragma unroll
         for (int j = 0; j < kSortHeld; ++j) {
             if (i0 + j * 32 >= hi) break;
-            const int e = held[j];
-            const unsigned peers = __match_any_sync(0xffffffffu, e);
-            if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-            __syncwarp();
+            if (held[j] >= 0) atomicAdd(&mine[held[j]], 1);  // whole numbers: the order does not matter
         }
     }
     __syncthreads();
     // per expert: exclusive prefix over the warps, and this CTA's total
     for (int e = threadIdx.x; e < B; e += blockDim.x) {
         int sum = 0;
-        for (int w = 0; w < kSortWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             const int c = s_hist[w * B + e];
             s_hist[w * B + e] = sum;
             sum += c;
@@ -122,7 +131,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
         __syncthreads();
         int base = carry;
         for (int w = 0; w < warp; ++w) base += s_warp[w];
-        for (int w = 0; w < kSortWarps; ++w) carry += s_warp[w];
+        for (int w = 0; w < warps; ++w) carry += s_warp[w];
         const int first = base + inc - all;
         if (e < B) {
             s_base[e] = first + before;
@@ -137,7 +146,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) order_kernel(OrderArgs a) {
         for (int j = 0; j < kSortHeld; ++j) {
             if (i0 + j * 32 >= hi) break;
             const int i = i0 + j * 32 + lane, e = held[j];
-            const unsigned peers = __match_any_sync(0xffffffffu, e);
+            const unsigned peers = same_expert(e, a.bits);
             if (e >= 0) {
                 const int row = s_base[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
                 a.row_of[i] = e == a.E ? -1 : row;
@@ -201,44 +210,66 @@ __device__ __forceinline__ void copy_row(const uint8_t* src, uint8_t* dst, int64
     }
 }
 
-// Blocks of tokens; each also clears its share of the rows behind the last expert's.
-template <bool ANY>
+__device__ __forceinline__ void clear_tail(const CopyArgs& a, int used, bool any) {
+    const int R = a.T * a.K;
+    for (int64_t r = max(0, min(used, R)) + int64_t(blockIdx.x); r < R; r += gridDim.x) {
+        if (any) copy_row<true>(nullptr, a.rows + r * a.bytes, a.bytes);
+        else copy_row<false>(nullptr, a.rows + r * a.bytes, a.bytes);
+        if (a.scale)
+            for (int c = threadIdx.x; c < a.n_scale; c += blockDim.x) a.srows[r * a.n_scale + c] = 0u;
+    }
+}
+
+// Rows of whole 16-byte pieces: a thread reads one piece of a token and stores it K times.  Pieces are numbered
+// through all tokens, so that narrow rows fill a CTA; every CTA also clears its share of the rows behind the
+// last expert's.
+__global__ void __launch_bounds__(256) sort_pieces_kernel(CopyArgs a, int pieces) {
+    chain_wait();
+    chain_release();
+    const int R = a.T * a.K;
+    const int64_t all = int64_t(a.T) * pieces, step = int64_t(gridDim.x) * blockDim.x;
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += step) {
+        const int t = int(i / pieces);
+        const int64_t at = (i - int64_t(t) * pieces) * 16;
+        const uint4 u = *reinterpret_cast<const uint4*>(a.x + t * a.ld_x + at);
+        const int32_t* row = a.row_of + int64_t(t) * a.K;
+#pragma unroll 8
+        for (int k = 0; k < a.K; ++k) {
+            const int r = __ldg(row + k);
+            if (unsigned(r) < unsigned(R)) *reinterpret_cast<uint4*>(a.rows + r * a.bytes + at) = u;
+        }
+    }
+    if (a.scale) {
+        const int64_t words = int64_t(a.T) * a.n_scale;
+        for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < words; i += step) {
+            const int t = int(i / a.n_scale), c = int(i - int64_t(t) * a.n_scale);
+            const uint32_t v = a.scale[t * a.ld_scale + c];
+            for (int k = 0; k < a.K; ++k) {
+                const int r = __ldg(a.row_of + int64_t(t) * a.K + k);
+                if (unsigned(r) < unsigned(R)) a.srows[int64_t(r) * a.n_scale + c] = v;
+            }
+        }
+    }
+    clear_tail(a, *a.rows_used, false);
+}
+
+// Rows of any length and place: one CTA a token.
 __global__ void __launch_bounds__(256) sort_rows_kernel(CopyArgs a) {
     chain_wait();
     chain_release();
     const int R = a.T * a.K;
     for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
         const int32_t* row = a.row_of + int64_t(t) * a.K;
-        const uint8_t* src = a.x + t * a.ld_x;
-        if (a.scale) {
-            for (int i = threadIdx.x; i < a.n_scale * a.K; i += blockDim.x) {
-                const int k = i / a.n_scale, c = i - k * a.n_scale, r = __ldg(row + k);
-                if (unsigned(r) < unsigned(R)) a.srows[int64_t(r) * a.n_scale + c] = a.scale[t * a.ld_scale + c];
-            }
-        }
-        if constexpr (ANY) {
-            for (int k = 0; k < a.K; ++k) {
-                const int r = __ldg(row + k);
-                if (unsigned(r) < unsigned(R)) copy_row<true>(src, a.rows + r * a.bytes, a.bytes);
-            }
-        } else {
-            // each piece is read once and stored K times
-            for (int64_t at = int64_t(threadIdx.x) * 16; at < a.bytes; at += int64_t(blockDim.x) * 16) {
-                const uint4 u = *reinterpret_cast<const uint4*>(src + at);
-#pragma unroll 4
-                for (int k = 0; k < a.K; ++k) {
-                    const int r = __ldg(row + k);
-                    if (unsigned(r) < unsigned(R)) *reinterpret_cast<uint4*>(a.rows + r * a.bytes + at) = u;
-                }
-            }
+        for (int k = 0; k < a.K; ++k) {
+            const int r = __ldg(row + k);
+            if (unsigned(r) >= unsigned(R)) continue;
+            copy_row<true>(a.x + t * a.ld_x, a.rows + r * a.bytes, a.bytes);
+            if (a.scale)
+                for (int c = threadIdx.x; c < a.n_scale; c += blockDim.x)
+                    a.srows[int64_t(r) * a.n_scale + c] = a.scale[t * a.ld_scale + c];
         }
     }
-    const int used = max(0, min(*a.rows_used, R));
-    for (int64_t r = used + int64_t(blockIdx.x); r < R; r += gridDim.x) {
-        copy_row<ANY>(nullptr, a.rows + r * a.bytes, a.bytes);
-        if (a.scale)
-            for (int c = threadIdx.x; c < a.n_scale; c += blockDim.x) a.srows[r * a.n_scale + c] = 0u;
-    }
+    clear_tail(a, *a.rows_used, true);
 }
 
 // ---- back to the tokens -----------------------------------------------------------------
@@ -438,8 +469,7 @@ __global__ void __launch_bounds__(256) unsort_grad_kernel(UnsortGradArgs a) {
             __syncthreads();
             if (threadIdx.x < kAhead && k0 + int(threadIdx.x) < a.K) {
                 float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += s_part[i][threadIdx.x];
+                for (int i = 0; i < int(blockDim.x >> 5); ++i) sum += s_part[i][threadIdx.x];  // fixed order
                 a.d_weight[int64_t(t) * a.K + k0 + threadIdx.x] = sum;  // 0 for an absent route
             }
             __syncthreads();
@@ -453,16 +483,18 @@ __global__ void __launch_bounds__(256) unsort_grad_kernel(UnsortGradArgs a) {
 }
 
 cudaError_t launch_order(const OrderArgs& a, cudaStream_t stream) {
-    const size_t smem = size_t(kSortWarps + 2) * (a.E + 1) * 4;
+    // A cluster counts 2048 routes a turn and costs about 1 us more than one CTA: 4096 routes 9.5 -> 6.6 us.
+    const int ranks = a.n > 1024 ? kSortMaxCluster : 1;
+    int warps = kSortMaxWarps;
+    while (warps > kSortMinWarps && int64_t(warps / 2) * ranks * 32 * 2 >= a.n) warps /= 2;  // two routes a lane or fewer
+    const size_t smem = size_t(warps + 2) * (a.E + 1) * 4;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
         if (e != cudaSuccess) return e;
     }
-    // one CTA counts 256 routes a warp without reading them twice; beyond that the cluster shares them
-    const int ranks = a.n > kSortWarps * 32 * kSortHeld / 2 ? kSortMaxCluster : 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ranks);
-    cfg.blockDim = dim3(kSortWarps * 32);
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -508,7 +540,9 @@ extern "C" int cst_sort_routes(const void* topk_idx, int32_t idx_bytes, int32_t 
                               n_experts, kSortMaxExperts, first_expert);
     if (!offsets || (T > 0 && (!topk_idx || !row_of || !route_of)))
         return set_last_error(CST_ERR_INVALID_ARG, "null index or output");
-    const OrderArgs a{topk_idx, idx_bytes == 8, T * K, n_experts, first_expert, row_of, route_of, offsets};
+    int bits = 1;
+    while ((n_experts >> (bits - 1)) != 0) ++bits;
+    const OrderArgs a{topk_idx, idx_bytes == 8, T * K, n_experts, first_expert, bits, row_of, route_of, offsets};
     return launched("sort_routes", launch_order(a, static_cast<cudaStream_t>(stream)));
 }
 
@@ -527,11 +561,18 @@ extern "C" int cst_sort_rows(const void* x, int64_t row_bytes, int64_t ld_bytes,
                      reinterpret_cast<uint32_t*>(rows_scale)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool aligned = row_bytes % 16 == 0 && rows_aligned16(x, ld_bytes, 1) && rows_aligned16(rows, row_bytes, 1);
-    // as many threads as a row has pieces, up to 256
     const int64_t pieces = (row_bytes + 15) / 16;
-    const int threads = pieces >= 256 ? 256 : int((pieces + 31) / 32 * 32);
-    const cudaError_t e = launch_chained(aligned ? sort_rows_kernel<false> : sort_rows_kernel<true>, dim3(T), dim3(threads),
-                                         0, s, a);
+    if (pieces > INT32_MAX) return set_last_error(CST_ERR_INVALID_ARG, "row_bytes=%lld is too long", (long long)row_bytes);
+    cudaError_t e;
+    if (aligned) {
+        const int64_t ctas = (T * pieces + 255) / 256;
+        e = launch_chained(sort_pieces_kernel, dim3(unsigned(ctas < INT32_MAX ? ctas : INT32_MAX)), dim3(256), 0, s, a,
+                           int(pieces));
+    } else {
+        // as many threads as a row has pieces, up to 256
+        const int threads = pieces >= 256 ? 256 : int((pieces + 31) / 32 * 32);
+        e = launch_chained(sort_rows_kernel, dim3(T), dim3(threads), 0, s, a);
+    }
     return launched("sort_rows", e);
 }
 
@@ -589,5 +630,7 @@ extern "C" int cst_unsort_rows_grad(const void* grad, int32_t grad_dtype, int64_
                   : rows_dtype == CST_DTYPE_BF16 ? unsort_grad_kernel<2, false>
                   : rows_dtype == CST_DTYPE_FP16 ? unsort_grad_kernel<1, false>
                                                  : unsort_grad_kernel<3, false>;
-    return launched("unsort_rows_grad", launch_chained(kernel, dim3(T), dim3(256), 0, s, a));
+    // as many threads as a row has vectors, up to 256
+    const int threads = H >= 2048 ? 256 : (H + 7) / 8 < 32 ? 32 : ((H + 7) / 8 + 31) / 32 * 32;
+    return launched("unsort_rows_grad", launch_chained(kernel, dim3(T), dim3(threads), 0, s, a));
 }

@@ -85,6 +85,7 @@ class Int4Weight:
         self.out_features = self.n // 2 if swiglu else self.n
         self.data = torch.zeros(size.value, dtype=torch.uint8, device=device)
         self.device = self.data.device
+        self._sizes: dict = {}  # bytes of a workspace by x's type and rows
 
     def load(self, expert: int, q: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None) -> None:
         """Lay expert ``expert``'s ``q [N, K / 2]``, ``scale`` and ``zero`` ``[N, K / group]`` out (stream-ordered)."""
@@ -107,6 +108,16 @@ class Int4Weight:
         with _on(self.device):
             check(_lib.lib.cst_int4_pack(self._ref, first, count, q.data_ptr(), scale.data_ptr(), _ptr(zero),
                                          self.data.data_ptr(), _stream(self.device)))
+
+    def _workspace(self, xt: int, R: int) -> int:
+        size = self._sizes.get((xt, R))
+        if size is None:
+            got = ctypes.c_int64()
+            check(_lib.lib.cst_int4_workspace(self._ref, xt, R, ctypes.byref(got)))
+            if len(self._sizes) >= 64:
+                self._sizes.clear()
+            size = self._sizes[(xt, R)] = got.value
+        return size
 
     def device_error(self) -> None:
         """Wait for the current stream and raise if a product's bounded device-side wait gave up."""
@@ -163,9 +174,7 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     lds = 0
     if x_scale is not None:
         x_scale, lds = _rows(x_scale)
-    size = ctypes.c_int64()
-    check(_lib.lib.cst_int4_workspace(w._ref, xt, R, ctypes.byref(size)))
-    room = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    room = torch.empty(w._workspace(xt, R), dtype=torch.uint8, device=dev)
     with _on(dev):
         check(_lib.lib.cst_grouped_int4(w._ref, w.data.data_ptr(), x.data_ptr(), xt, ldx, _ptr(x_scale), lds,
                                         _ptr(offsets), R, room.data_ptr(), out.data_ptr(), ot, w.out_features,

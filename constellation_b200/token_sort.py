@@ -29,13 +29,22 @@ from ._lib import check
 from .context import _on, _ptr, _rows, _stream, dtype_code
 
 
-@dataclass
+@dataclass(frozen=True)
 class TokenOrder:
-    """Routes in the order (expert, token, k), as ``sort_routes`` makes it (int32, on one device)."""
+    """Routes in the order (expert, token, k), as ``sort_routes`` makes it: contiguous int32 on one device."""
 
     row_of: torch.Tensor    # [T, K] row of a route, -1 where its expert is held elsewhere
     route_of: torch.Tensor  # [T * K] t * K + k of a row, -1 behind the last expert's rows
     offsets: torch.Tensor   # [n_experts + 1] first row of each expert; the last entry: rows in use
+
+    def __post_init__(self):
+        r, q, o = self.row_of, self.route_of, self.offsets
+        if r.dim() != 2 or q.dim() != 1 or o.dim() != 1 or q.shape[0] != r.numel() or o.shape[0] < 2:
+            raise RuntimeError("not an order: row_of [T, K], route_of [T * K] and offsets [n_experts + 1] are expected")
+        dev = r.device
+        for t in (r, q, o):
+            if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+                raise RuntimeError("an order is contiguous int32 on one device")
 
 
 def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0) -> TokenOrder:
@@ -53,7 +62,7 @@ def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0
     n_experts = int(n_experts)
     if not 1 <= n_experts <= 1024:
         raise ValueError(f"n_experts must be in [1, 1024], got {n_experts}")
-    row_of = torch.empty((T, K), dtype=torch.int32, device=dev)
+    row_of = torch.empty_like(topk_idx, dtype=torch.int32)
     route_of = torch.empty(n, dtype=torch.int32, device=dev)
     offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
     with _on(dev):
@@ -63,14 +72,9 @@ def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0
     return TokenOrder(row_of, route_of, offsets)
 
 
-def _check_order(order: TokenOrder, dev: torch.device) -> tuple[int, int]:
-    r, q, o = order.row_of, order.route_of, order.offsets
-    if r.dim() != 2 or q.dim() != 1 or o.dim() != 1 or q.shape[0] != r.shape[0] * r.shape[1] or o.shape[0] < 2:
-        raise RuntimeError("not an order: row_of [T, K], route_of [T * K] and offsets [n_experts + 1] are expected")
-    for t in (r, q, o):
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-            raise RuntimeError("an order is contiguous int32 on the device of the rows")
-    return r.shape[0], r.shape[1]
+def _check_order(order: TokenOrder, dev: torch.device) -> None:
+    if order.row_of.device != dev:
+        raise RuntimeError(f"device mismatch: rows={dev} order={order.row_of.device}")
 
 
 def _matrix(name: str, t: torch.Tensor, rows: int) -> None:
