@@ -9,10 +9,11 @@
 // even steps.  So a pair of logic operations turns 8 packed weights into 8 operands of the 8-bit
 // matrix product, and the zero point is one more product of the same x with a constant operand,
 //     2^-9 sum (q - z) x = sum (q 2^-9) x + sum (-z 2^-9) x,
-// into the same accumulator.  x enters as e4m3 terms, x = s (t1 + t2 / 16 + t3 / 256) with a power of two s that
-// fits the largest |x| of the row: two terms for bf16 (8 bits = 4 + 4), three for fp16 (11 bits); what
-// they drop is below 2^-21 (bf16) or 2^-25 (fp16) of that largest |x|.  e4m3 rows enter as they are, with
-// their scales.  The products are exact and the sums fp32, with one rounding at the end.
+// into the same accumulator.  x enters as e4m3 terms with a power of two s that fits the largest |x| of the
+// row to 448: two terms for bf16 (8 bits = 4 + 4), x = s (t1 + t2 / 16), three for fp16 (11 bits),
+// x = s (t1 + t2 + t3 / 512).  They are x exactly where |x| is above 2^-13 (bf16) or 2^-11 (fp16) of that
+// largest; below, what they drop is less than 2^-21 (2^-22) of the largest.  e4m3 rows enter as they are,
+// with their scales.  The products are exact and the sums fp32, with one rounding at the end.
 //
 // Layout of one weight (written once by pack_kernel): blocks of 128 weight rows, each a run of
 // chunks of 128 k; a chunk is 8192 bytes of q, then the 128 rows' scales [128 / group][128], then
@@ -110,7 +111,8 @@ __global__ void __launch_bounds__(256) pack_kernel(Geom g, const uint8_t* q, con
 
 constexpr int kFactBytes = 16;  // of an e4m3 row and chunk: its scale, padded to what a bulk copy takes
 
-// One CTA a row.  terms: [rows * TERMS][chunks * 128], columns past k zero.  facts: the rows' s; for e4m3
+// One CTA a row.  terms: [rows * TERMS][chunks * 128] (of three terms [t1, t3, t2][rows][chunks * 128], so that one
+// product takes t1 and t3), columns past k zero.  facts: the rows' s; for e4m3
 // (TERMS 1) [chunks][rows] of x_scale, 16 bytes each.  A row's first 8192 columns stay in registers between
 // its maximum and its terms; more are read twice.
 template <int TERMS>
@@ -186,17 +188,19 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
         for (int j = 0; j < 8; ++j) v[j] = x8[j] * inv;
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) {
+            // exact: the rest has fewer bits than v; its largest is 16 after the first term, which 16-fold stays
+            // below 448, and 1/2 after the second of three, which does so 512-fold
+            const float up = TERMS == 2 ? 16.0f : t == 0 ? 1.0f : 512.0f;
             uint32_t q[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 q[j] = e4m3x2_rn(v[2 * j], v[2 * j + 1]);
                 const float2 f = e4m3x2_to_f32x2(q[j]);
-                // exact: the rest has fewer bits than v; its largest is 16, which 16-fold stays below 448
-                v[2 * j] = (v[2 * j] - f.x) * 16.0f;
-                v[2 * j + 1] = (v[2 * j + 1] - f.y) * 16.0f;
+                v[2 * j] = (v[2 * j] - f.x) * up;
+                v[2 * j + 1] = (v[2 * j + 1] - f.y) * up;
             }
-            *reinterpret_cast<uint2*>(terms + (r * TERMS + t) * width + c) =
-                make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+            const int64_t at_row = TERMS == 2 ? r * 2 + t : (t == 0 ? 0 : 3 - t) * int64_t(rows) + r;
+            *reinterpret_cast<uint2*>(terms + at_row * width + c) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
         }
     };
 #pragma unroll
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
 //              product's A operand (and the row's zero points, if there are any);
 //   warp 1     one lane issues the tcgen05 products, a fresh fp32 accumulator for each group;
 //   the last   output warps, as many sets: each thread owns a weight row of the accumulators:
-//              acc[t] += 2^9 scale * (D1[t] + D2[t] / 16 + D3[t] / 256), and at the end of an item the results.
+//              acc[t] += 2^9 scale * (D1[t] + D2[t] / 16), and at the end of an item the results.
 // So each weight byte is read once from HBM and once from shared memory, and never goes back there.
 
 constexpr int kMaxStages = 12;
@@ -231,6 +235,12 @@ constexpr int kThreads = (kWarpOut + 4 * kSets) * 32;
 constexpr int kMaxBufs = 4;                     // steps in tensor memory
 constexpr int kACols = kChunk / 4;              // columns of A: [128 rows][128 k] of 8 bits
 constexpr int kMostColumns = 512 / 2 - kACols - 32;  // accumulator columns of a chunk with which two steps fit
+
+// Columns of tensor memory of an accumulator: [rows][terms], for three terms [2][rows], of which the first
+// takes two.  A product is a multiple of 16 wide.
+__host__ __device__ constexpr int acc_columns(int terms, int tile) {
+    return terms == 3 ? 2 * (tile < 16 ? 16 : tile) : (tile * terms + 15) / 16 * 16;
+}
 
 struct Int4Args {
     Geom g;
@@ -250,7 +260,7 @@ struct Int4Args {
     int step;         // chunks of a step
     int bufs;         // steps in tensor memory: A, behind all of them the zero points, then the accumulators
     int z_at, d_at;   // first columns of the zero points (8 for each group of a step, or 8 in all) and accumulators
-    int d_cols;       // columns of one accumulator: tile * TERMS up to a multiple of 16
+    int d_cols;       // acc_columns
 };
 
 __device__ __forceinline__ float scale_at(const uint8_t* scales, int dtype, int s) {
@@ -263,6 +273,15 @@ __device__ __forceinline__ float scale_at(const uint8_t* scales, int dtype, int 
 __device__ __forceinline__ void tma_box_g2s(void* dst, const CUtensorMap* map, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// The same of three planes of rows.
+__device__ __forceinline__ void tma_planes_g2s(void* dst, const CUtensorMap* map, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4}], [%5];\n" ::"r"(
             smem_u32(dst)),
         "l"(map), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
@@ -496,7 +515,7 @@ __device__ __forceinline__ void producer_role(const Int4Args& a, Shared& sh, con
         const Item it = find_item(a, sh.tile, sh.row, i);
         const uint8_t* w = a.data + it.expert * a.g.expert_bytes() +
                            (int64_t(it.block) * a.g.chunks + int64_t(sp.step0) * a.step) * a.g.chunk_bytes;
-        const int x_row = it.row * TERMS;
+        const int x_row = TERMS == 2 ? it.row * 2 : it.row;
         for (int c = sp.step0; c < sp.step1; ++c) {
             if (!lane_wait(&sh.empty[s.i], s.phase ^ 1, a.err)) goto out;
             uint8_t* stage = s_ring + s.i * a.stage_bytes;
@@ -510,7 +529,8 @@ __device__ __forceinline__ void producer_role(const Int4Args& a, Shared& sh, con
                 chain_wait();
                 waiting = false;
             }
-            tma_box_g2s(stage, &xmap, x_row, c * a.step, &sh.full[s.i]);
+            if constexpr (TERMS == 3) tma_planes_g2s(stage, &xmap, x_row, c * a.step, &sh.full[s.i]);
+            else tma_box_g2s(stage, &xmap, x_row, c * a.step, &sh.full[s.i]);
             if constexpr (TERMS == 1)
                 for (int h = 0; h < n; ++h)
                     tma_bulk_g2s(stage + a.f_at + h * a.tile * kFactBytes,
@@ -587,7 +607,8 @@ __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const 
 // through a lane that the compiler does not know to be alone it took 160.
 template <int TERMS, int GROUPS, int TILE, bool ZERO>
 __device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Span& sp) {
-    constexpr uint32_t kD = (TILE * TERMS + 15) / 16 * 16;  // columns of an accumulator
+    constexpr uint32_t kD = acc_columns(TERMS, TILE);       // columns of an accumulator
+    constexpr uint32_t kPlane = TILE * kChunk / 16;         // bytes of a term of three, over 16
     constexpr uint32_t kX = TILE * TERMS * kChunk / 16;     // bytes of x of a chunk, over 16
     Ring s, b;
     int used = 0;
@@ -595,7 +616,9 @@ __device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Sp
     const uint32_t x_step = uint32_t(a.stage_bytes) >> 4;
     for (int64_t i = sp.first; i < sp.items; i += sp.step) {
         const Item it = find_item(a, sh.tile, sh.row, i);
-        const uint32_t idesc = umma_idesc_e4m3(128, (it.rows * TERMS + 15) / 16 * 16);
+        // three terms: the first and the third side by side, then the second onto the first
+        const uint32_t idesc = umma_idesc_e4m3(128, TERMS == 3 ? kD / (TILE < 16 ? 2 : 1) : (it.rows * TERMS + 15) / 16 * 16);
+        const uint32_t idesc2 = umma_idesc_e4m3(128, kD / 2);
         for (int c = sp.step0; c < sp.step1; ++c) {
             // A is written, and so the stage with its x is full; the accumulators are free
             if (!lane_wait(&sh.ready[b.i], b.phase, a.err)) goto out;
@@ -611,8 +634,17 @@ __device__ __forceinline__ void mma_role(const Int4Args& a, Shared& sh, const Sp
                 for (int ks = 0; ks < 4; ++ks) {  // 32 k
                     const uint32_t g = h * GROUPS + ks / (4 / GROUPS);
                     const uint64_t xk = x + h * kX + ks * 2;
-                    tc_mma_ts(d + g * kD, w + h * kACols + ks * 8, xk, idesc, ks % (4 / GROUPS) > 0);
-                    tc_mma_ts(d + g * kD, ZERO ? z + g * 8 : z, xk, idesc, true);
+                    const uint32_t dg = d + g * kD, wk = w + h * kACols + ks * 8, zk = ZERO ? z + g * 8 : z;
+                    tc_mma_ts(dg, wk, xk, idesc, ks % (4 / GROUPS) > 0);
+                    tc_mma_ts(dg, zk, xk, idesc, true);
+                    if constexpr (TERMS == 3) {
+                        if constexpr (TILE < 16) {  // a product is 16 rows wide at least, so the third has its own
+                            tc_mma_ts(dg + kD / 2, wk, xk + kPlane, idesc, ks % (4 / GROUPS) > 0);
+                            tc_mma_ts(dg + kD / 2, zk, xk + kPlane, idesc, true);
+                        }
+                        tc_mma_ts(dg, wk, xk + 2 * kPlane, idesc2, true);
+                        tc_mma_ts(dg, zk, xk + 2 * kPlane, idesc2, true);
+                    }
                 }
             }
             tc_commit(&sh.done[b.i]);
@@ -626,12 +658,14 @@ out:
     for (int j = 0; j < used; ++j) lane_wait(&sh.done[j], j < b.i ? b.phase : b.phase ^ 1, a.err);
 }
 
-// N (a multiple of 8) columns from `d` of this thread's lane of tensor memory.
-template <int N>
-__device__ __forceinline__ void load_columns(uint32_t d, uint32_t (&v)[N]) {
-#pragma unroll
-    for (int j = 0; j + 16 <= N; j += 16) tmem_ld16(d + j, v + j);
-    if constexpr (N % 16) tmem_ld8(d + N - 8, v + N - 8);
+// The columns of N rows (8 or 16) from `d` of this thread's lane of tensor memory; of three terms the second half
+// lies `half` columns on.
+template <int TERMS, int N>
+__device__ __forceinline__ void load_piece(uint32_t d, int half, uint32_t* v) {
+    if constexpr (TERMS * N == 8 || TERMS == 3) tmem_ld8(d, v);
+    else tmem_ld16(d, v);
+    if constexpr (TERMS == 3) tmem_ld8(d + half, v + 8);
+    static_assert(TERMS == 1 ? N == 8 || N == 16 : N == 8, "a piece is 8 or 16 columns");
 }
 
 // One item: the sums of ROWS rows of x over the steps of this set of output warps, for this thread's weight
@@ -639,9 +673,9 @@ __device__ __forceinline__ void load_columns(uint32_t d, uint32_t (&v)[N]) {
 template <int TERMS, int GROUPS, int ROWS>
 __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, int row, uint32_t lanes,
                                            Ring& s, Ring& b, int& turn, float (&acc)[ROWS]) {
-    // rows whose columns are in registers at a time
-    constexpr int kCols = 16, kFit = kCols / TERMS / 8 * 8 > 8 ? kCols / TERMS / 8 * 8 : 8;
-    constexpr int kAt = ROWS < kFit ? ROWS : kFit, kGo = kAt == ROWS && kAt * TERMS <= kCols ? kCols / (kAt * TERMS) : 1;
+    // a row's columns; rows whose columns are in registers at a time
+    constexpr int kAccs = TERMS == 1 ? 1 : 2, kCols = 16, kFit = kCols / kAccs;
+    constexpr int kAt = ROWS < kFit ? ROWS : kFit, kGo = kAt == ROWS && kAt * kAccs < kCols ? kCols / (kAt * kAccs) : 1;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) acc[t] = 0.0f;
@@ -659,11 +693,11 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
         // (chunk, group) pieces, kGo of them at a time while their columns fit in registers
 #pragma unroll 1
         for (int p = 0; p < n; p += kGo, d += kGo * a.d_cols) {
-            uint32_t v[kGo][kAt * TERMS];
+            uint32_t v[kGo][kAt * kAccs];
             float scale[kGo];
 #pragma unroll
             for (int k = 0; k < kGo; ++k)
-                if (k == 0 || p + k < n) load_columns<kAt * TERMS>(d + k * a.d_cols, v[k]);
+                if (k == 0 || p + k < n) load_piece<TERMS, kAt>(d + k * a.d_cols, a.d_cols / 2, v[k]);
 #pragma unroll
             for (int k = 0; k < kGo; ++k) {
                 const int q = min(p + k, n - 1);
@@ -672,7 +706,7 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
             }
 #pragma unroll
             for (int t0 = 0; t0 < ROWS; t0 += kAt) {
-                if (t0 > 0) load_columns<kAt * TERMS>(d + t0 * TERMS, v[0]);  // then kGo is 1
+                if (t0 > 0) load_piece<TERMS, kAt>(d + (TERMS == 2 ? 2 * t0 : t0), a.d_cols / 2, v[0]);  // then kGo is 1
                 tmem_wait_ld();
 #pragma unroll
                 for (int k = 0; k < kGo; ++k) tmem_reg_fence(v[k]);
@@ -681,9 +715,12 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
                     if (k > 0 && p + k >= n) break;
 #pragma unroll
                     for (int t = 0; t < kAt; ++t) {
-                        float y = __uint_as_float(v[k][t * TERMS + TERMS - 1]);
-#pragma unroll
-                        for (int j = TERMS - 2; j >= 0; --j) y = fmaf(y, 0.0625f, __uint_as_float(v[k][t * TERMS + j]));
+                        float y;
+                        if constexpr (TERMS == 1) y = __uint_as_float(v[k][t]);
+                        if constexpr (TERMS == 2)
+                            y = fmaf(__uint_as_float(v[k][2 * t + 1]), 0.0625f, __uint_as_float(v[k][2 * t]));
+                        if constexpr (TERMS == 3)
+                            y = fmaf(__uint_as_float(v[k][kAt + t]), 1.0f / 512, __uint_as_float(v[k][t]));
                         if constexpr (TERMS == 1)
                             y *= *reinterpret_cast<const float*>(stage + a.f_at + ((p + k) / GROUPS * a.tile + t0 + t) * kFactBytes);
                         acc[t0 + t] = fmaf(y, scale[k], acc[t0 + t]);
@@ -906,8 +943,8 @@ int64_t terms_bytes(const Geom& g, int terms, int64_t R) {
 template <int TERMS, int GROUPS>
 int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
     constexpr int kShared = 216 * 1024;
-    a.tile = choose_tile(a.R, a.g.E, TERMS * GROUPS);
-    a.d_cols = (a.tile * TERMS + 15) / 16 * 16;
+    a.tile = choose_tile(a.R, a.g.E, (TERMS == 1 ? 1 : 2) * GROUPS);
+    a.d_cols = acc_columns(TERMS, a.tile);
     // tensor memory: of a chunk, and once for a constant zero point
     const int cols = kACols + (a.d_cols + (a.g.has_zero ? 8 : 0)) * GROUPS, once = a.g.has_zero ? 0 : 8;
     for (a.step = kMaxStep; a.step > 1 && (512 - once) / (a.step * cols) < 2;) --a.step;
@@ -931,11 +968,13 @@ int launch_int4(Int4Args a, void* workspace, int sms, cudaStream_t stream) {
     CUtensorMap map;
     const EncodeTiled encode = encode_tiled();
     if (!encode) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    // [chunk][row and term][128 columns of the chunk]
-    const cuuint64_t dims[3] = {kChunk, cuuint64_t(a.R) * TERMS, cuuint64_t(a.g.chunks)};
-    const cuuint64_t strides[2] = {dims[2] * kChunk, kChunk};
-    const cuuint32_t box[3] = {kChunk, cuuint32_t(a.tile * TERMS), cuuint32_t(a.step)}, steps[3] = {1, 1, 1};
-    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, workspace, dims, strides, box, steps,
+    // [chunk][row and term][128 columns of the chunk], of three terms [chunk][term][row][128 columns]
+    const cuuint64_t chunks = a.g.chunks, width = chunks * kChunk, R = a.R;
+    const cuuint32_t tile = a.tile, step = a.step, ones[4] = {1, 1, 1, 1};
+    const cuuint64_t dims[4] = {kChunk, TERMS == 3 ? R : R * TERMS, TERMS == 3 ? 3 : chunks, chunks};
+    const cuuint64_t strides[3] = {width, TERMS == 3 ? R * width : kChunk, kChunk};
+    const cuuint32_t box[4] = {kChunk, TERMS == 3 ? tile : tile * TERMS, TERMS == 3 ? 3 : step, step};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, TERMS == 3 ? 4 : 3, workspace, dims, strides, box, ones,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_last_error(CST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
