@@ -331,7 +331,7 @@ int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int32_t R, int
  *   workspace  cst_int4_workspace bytes, 16-byte aligned, of this call alone until it is done
  *   out  [R, n] (n / 2 with swiglu) in out_dtype (fp16, bf16, fp32)
  * x enters the products as 8-bit terms that hold it exactly but for what is below 2^-21 (bf16) or
- * 2^-25 (fp16) of the largest |x| of its row; sums are fp32, with one rounding.
+ * 2^-22 (fp16) of the largest |x| of its row; sums are fp32, with one rounding.
  * An infinity in a row of x makes the row's results NaN.  `data` is only read, but for its error word. */
 int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
                      const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* workspace,

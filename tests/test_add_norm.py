@@ -130,6 +130,39 @@ def test_strides_and_offsets(H, offset, stride):
 
 
 @gpu
+@pytest.mark.parametrize("T,H,offset,stride", [(640, 8, 0, 8), (640, 250, 0, 256), (700, 256, 8, 272), (1300, 2048, 0, 2048),
+                                               (640, 8192, 0, 8192), (640, 5001, 1, 5003), (3, 9001, 1, 9003),
+                                               (640, 9001, 0, 9001), (700, 8200, 0, 8200)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_many_rows(T, H, offset, stride, dt):
+    """Long batches go from row to row: a row's numbers reach no other row, with and without what is optional."""
+    from constellation_b200.context import add_rms_norm, add_rms_norm_fp8
+
+    g = torch.Generator().manual_seed(H)
+    x = (torch.randn(T, stride + 8, generator=g) * 2).to("cuda", dt)[:, offset:offset + H]
+    res = torch.randn(T, stride + 8, generator=g).to("cuda", dt)[:, offset:offset + H]
+    w = (1 + 0.1 * torch.randn(H, generator=g)).cuda()
+    h, y = formula(x, res, w)
+    room = torch.full((T, stride + 8), 7.0, device="cuda", dtype=dt)
+    out, s = add_rms_norm(x, res, w, out=room[:, offset:offset + H])
+    close(out, y, dt)
+    close(s, h, dt)
+    assert (room[:, :offset] == 7).all() and (room[:, offset + H:] == 7).all()
+    q, scale, s8 = add_rms_norm_fp8(x, res, w)
+    check8(q, scale, y)
+    assert torch.equal(s8, s)
+    bad = x.clone()
+    bad[T // 2] = math.nan
+    keep = torch.arange(T, device="cuda") != T // 2
+    q1, scale1, _ = add_rms_norm_fp8(bad, res, w)
+    assert torch.equal(q1.view(torch.uint8)[keep], q.view(torch.uint8)[keep]) and torch.equal(scale1[keep], scale[keep])
+    _, y0 = formula(x, None, None)
+    q, scale, none = add_rms_norm_fp8(x)
+    assert none is None
+    check8(q, scale, y0)
+
+
+@gpu
 def test_in_place():
     from constellation_b200.context import add_rms_norm, add_rms_norm_fp8
 
