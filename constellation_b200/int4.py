@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import CST_DTYPE_E4M3, check
-from .context import (ExpertContext, MoEConfig, _no_grad, _on, _ptr, _rows, _stream, dtype_code)
+from .context import (ExpertContext, MoEConfig, _empty, _no_grad, _on, _ptr, _rows, _stream, dtype_code)
 from .fp8_utils import dequant_fp8_weight_blockwise
 from .token_sort import sort_routes, sort_tokens, unsort_tokens
 
@@ -134,7 +134,11 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     leaves them, sorted by ``sort_tokens``).  ``offsets`` is int32 ``[E + 1]`` on the device, ascending
     (``TokenOrder.offsets``); without it there is one weight and it takes every row.  The result is
     ``[R, N]`` (``[R, N / 2]`` with swiglu) in ``out_dtype``: fp16, bf16 or fp32; by default ``x``'s type, bf16
-    for e4m3 rows.  fp32 sums, one rounding."""
+    for e4m3 rows.  ``out`` may not overlap ``x``.
+
+    fp32 sums, one rounding.  fp16 and bf16 rows enter as 8-bit terms: exactly where a number is above 2^-11 (fp16)
+    or 2^-13 (bf16) of its row's largest, and with an error below 2^-22 (2^-21) of that largest elsewhere.  So a row
+    whose outlier is 2^20 times the rest keeps little of the rest.  An infinity makes its row's results NaN."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda:
         raise TypeError("grouped_int4 expects a 2-D CUDA tensor")
     dev = x.device
@@ -165,16 +169,20 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     else:
         offsets = offsets.contiguous()
     if out is None:
-        out = torch.empty((R, w.out_features),
-                          dtype=out_dtype or (torch.bfloat16 if xt == CST_DTYPE_E4M3 else x.dtype), device=dev)
-    elif out.shape != (R, w.out_features) or out.device != dev or not out.is_contiguous():
-        raise RuntimeError(f"out must be contiguous [{R}, {w.out_features}] on the device of x")
+        out = _empty(R, w.out_features, out_dtype or (torch.bfloat16 if xt == CST_DTYPE_E4M3 else x.dtype), dev)
+    elif (out.shape != (R, w.out_features) or out.device != dev or not out.is_contiguous()
+          or out_dtype not in (None, out.dtype)):
+        raise RuntimeError(f"out must be contiguous [{R}, {w.out_features}] on the device of x, of the out_dtype given")
+    elif R and x.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+        first, last = x.data_ptr(), x.data_ptr() + ((R - 1) * x.stride(0) + K) * x.element_size()
+        if out.data_ptr() < last and first < out.data_ptr() + out.numel() * out.element_size():
+            raise RuntimeError("out overlaps x, whose rows are still read while results are written")
     ot = dtype_code(out.dtype)
     x, ldx = _rows(x)
     lds = 0
     if x_scale is not None:
         x_scale, lds = _rows(x_scale)
-    room = torch.empty(w._workspace(xt, R), dtype=torch.uint8, device=dev)
+    room = torch.empty_strided((w._workspace(xt, R),), (1,), dtype=torch.uint8, device=dev)
     with _on(dev):
         check(_lib.lib.cst_grouped_int4(w._ref, w.data.data_ptr(), x.data_ptr(), xt, ldx, _ptr(x_scale), lds,
                                         _ptr(offsets), R, room.data_ptr(), out.data_ptr(), ot, w.out_features,

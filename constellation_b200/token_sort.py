@@ -26,7 +26,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check
-from .context import _on, _ptr, _rows, _stream, dtype_code
+from .context import _empty, _on, _ptr, _rows, _stream, dtype_code
 
 
 @dataclass(frozen=True)
@@ -62,9 +62,9 @@ def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0
     n_experts = int(n_experts)
     if not 1 <= n_experts <= 1024:
         raise ValueError(f"n_experts must be in [1, 1024], got {n_experts}")
-    row_of = torch.empty_like(topk_idx, dtype=torch.int32)
-    route_of = torch.empty(n, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    row_of = _empty(T, K, torch.int32, dev)
+    route_of = torch.empty_strided((n,), (1,), dtype=torch.int32, device=dev)
+    offsets = torch.empty_strided((n_experts + 1,), (1,), dtype=torch.int32, device=dev)
     with _on(dev):
         check(_lib.lib.cst_sort_routes(topk_idx.data_ptr(), topk_idx.element_size(), T, K, n_experts,
                                        int(first_expert), row_of.data_ptr(), route_of.data_ptr(), offsets.data_ptr(),
@@ -85,7 +85,7 @@ def _matrix(name: str, t: torch.Tensor, rows: int) -> None:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
 
 
 def _refuse_capture(what: str) -> None:
@@ -104,12 +104,12 @@ def _sort(x, order, scale):
     H, dev = x.shape[1], x.device
     x, ld = _rows(x)
     size = x.element_size()
-    rows = torch.empty((T * K, H), dtype=x.dtype, device=dev)
+    rows = _empty(T * K, H, x.dtype, dev)
     rows_scale, n_scale, ld_scale = None, 0, 0
     if scale is not None:
         scale, ld_scale = _rows(scale)
         n_scale = scale.shape[1]
-        rows_scale = torch.empty((T * K, n_scale), dtype=torch.float32, device=dev)
+        rows_scale = _empty(T * K, n_scale, torch.float32, dev)
     with _on(dev):
         check(_lib.lib.cst_sort_rows(x.data_ptr(), H * size, ld * size, _ptr(scale), n_scale, ld_scale, T, K,
                                      order.row_of.data_ptr(), _end(order), rows.data_ptr(), _ptr(rows_scale),
@@ -125,7 +125,7 @@ def _unsort(rows, order, weight, residual, out_dtype):
     if residual is not None:
         residual, ldr = _rows(residual)
         rt = dtype_code(residual.dtype)
-    out = torch.empty((T, H), dtype=out_dtype, device=dev)
+    out = _empty(T, H, out_dtype, dev)
     with _on(dev):
         check(_lib.lib.cst_unsort_rows(rows.data_ptr(), dtype_code(rows.dtype), ld, order.row_of.data_ptr(),
                                        _ptr(weight), T, K, H, _ptr(residual), rt, ldr, out.data_ptr(),
@@ -260,8 +260,8 @@ def _unsort_grad(grad, rows, rows_dtype, order, weight, need_rows, need_weight):
     ld_rows = 0
     if rows is not None:
         rows, ld_rows = _rows(rows)
-    d_rows = torch.empty((T * K, H), dtype=rows_dtype, device=dev) if need_rows else None
-    d_weight = torch.empty((T, K), dtype=torch.float32, device=dev) if need_weight else None
+    d_rows = _empty(T * K, H, rows_dtype, dev) if need_rows else None
+    d_weight = _empty(T, K, torch.float32, dev) if need_weight else None
     with _on(dev):
         check(_lib.lib.cst_unsort_rows_grad(grad.data_ptr(), dtype_code(grad.dtype), ld_grad, _ptr(rows),
                                             dtype_code(rows_dtype), ld_rows, order.row_of.data_ptr(), _ptr(weight),

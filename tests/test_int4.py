@@ -510,6 +510,8 @@ def test_refusals_of_device_tensors():
            lambda: grouped_int4(x8, w, off), lambda: grouped_int4(x, w, off, x_scale=xs),
            lambda: grouped_int4(x8, w, off, x_scale=xs[:, :1]), lambda: grouped_int4(x, w, off.cpu()),
            lambda: grouped_int4(x, w, off, out=torch.empty(4, 63, device="cuda")),
+           lambda: grouped_int4(x, w, off, out=torch.empty(4, 64, device="cuda"), out_dtype=torch.bfloat16),
+           lambda: grouped_int4(x, w, off, out=x.view(-1)[:256].view(4, 64)),
            lambda: grouped_int4(x.clone().requires_grad_(), w, off)]
     for f in bad:
         with pytest.raises(RuntimeError):
