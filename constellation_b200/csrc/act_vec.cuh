@@ -86,25 +86,38 @@ __device__ __forceinline__ void store8(void* base, int dtype, int64_t i, const f
     }
 }
 
-// 16 bytes from any address; the aligned 16-byte pieces that hold them have to be readable.
-__device__ __forceinline__ uint4 load16_any(const uint8_t* p) {
-    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
-    const uint4* q = reinterpret_cast<const uint4*>(p - off);
-    const uint4 lo = q[0];
-    if (off == 0) return lo;
-    const uint4 hi = q[1];
-    const bool two = off & 8u, one = off & 4u;
-    const uint32_t a0 = two ? lo.z : lo.x, a1 = two ? lo.w : lo.y, a2 = two ? hi.x : lo.z, a3 = two ? hi.y : lo.w,
-                   a4 = two ? hi.z : hi.x, a5 = two ? hi.w : hi.y;
-    const uint32_t b0 = one ? a1 : a0, b1 = one ? a2 : a1, b2 = one ? a3 : a2, b3 = one ? a4 : a3, b4 = one ? a5 : a4;
-    const uint32_t s = (off & 3u) * 8u;
-    return make_uint4(__funnelshift_r(b0, b1, s), __funnelshift_r(b1, b2, s), __funnelshift_r(b2, b3, s),
-                      __funnelshift_r(b3, b4, s));
+// The aligned 16-byte pieces around the 16 bytes at p, which it is cut from once they are there.
+struct Around {
+    uint4 lo, hi;
+    uint32_t off;
+    __device__ __forceinline__ uint4 piece() const {
+        const bool two = off & 8u, one = off & 4u;
+        const uint32_t a0 = two ? lo.z : lo.x, a1 = two ? lo.w : lo.y, a2 = two ? hi.x : lo.z, a3 = two ? hi.y : lo.w,
+                       a4 = two ? hi.z : hi.x, a5 = two ? hi.w : hi.y;
+        const uint32_t b0 = one ? a1 : a0, b1 = one ? a2 : a1, b2 = one ? a3 : a2, b3 = one ? a4 : a3, b4 = one ? a5 : a4;
+        const uint32_t s = (off & 3u) * 8u;
+        return make_uint4(__funnelshift_r(b0, b1, s), __funnelshift_r(b1, b2, s), __funnelshift_r(b2, b3, s),
+                          __funnelshift_r(b3, b4, s));
+    }
+};
+__device__ __forceinline__ Around load_around(const void* p) {
+    Around a;
+    a.off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) - a.off);
+    a.lo = q[0];
+    a.hi = a.off ? q[1] : make_uint4(0, 0, 0, 0);
+    return a;
 }
+
+// Whether the pieces around elements c .. c + 7 of a row of 16-bit elements lie in the row.
+__device__ __forceinline__ bool inner8(int c, int H) { return c >= 8 && c + 16 <= H; }
+
+// 16 bytes from any address; the aligned 16-byte pieces that hold them have to be readable.
+__device__ __forceinline__ uint4 load16_any(const uint8_t* p) { return load_around(p).piece(); }
 
 // Elements c .. c + 7 of a row of H elements at `row` (its first element's index), zero outside [0, H).
 __device__ __forceinline__ void load8_any(const void* base, int dtype, int64_t row, int c, int H, float (&v)[8]) {
-    if (c >= 8 && c + 16 <= H) {  // the pieces around these 8 lie in the row
+    if (inner8(c, H)) {
         const uint8_t* p = static_cast<const uint8_t*>(base) + (row + c) * (dtype == 3 ? 4 : 2);
         if (dtype == 3) {
             unpack4(load16_any(p), v);
