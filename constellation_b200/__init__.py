@@ -10,6 +10,9 @@ behind the reference's interfaces:
   ``combine_outputs_torch``), plus batched variants;
 * ``constellation_b200.fp8_utils`` / ``expert_placement`` -- the helper modules of the
   same names;
+* ``constellation_b200.token_sort`` -- tokens sorted by expert and back, with gradients;
+  ``constellation_b200.int4`` -- experts in 4 bits; ``context.add_rms_norm(_fp8)`` --
+  residual add and RMSNorm in one pass;
 * ``include/constellation_b200.h`` -- the C ABI that the reference node's
   ``BackendWorkspaceV2`` / ``BackendRegistryEntryV2`` hooks bind to.
 
@@ -17,4 +20,5 @@ The CUDA library is loaded lazily by the modules that need it, so the pure host
 helpers import without a GPU.
 """
 
-__all__ = ["context", "moe_layer_runtime", "fp8_utils", "expert_placement", "synthetic"]
+__all__ = ["context", "moe_layer_runtime", "fp8_utils", "expert_placement", "synthetic", "token_sort",
+           "int4"]
