@@ -101,6 +101,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
 
 
 _SAME_DEVICE = contextlib.nullcontext()
+_MOST_ROWS = 1 << 30
 
 
 def _on(device: torch.device):
@@ -134,6 +135,8 @@ def _add_rms_norm(what, x, residual, weight, eps, sum_out, out, out_dtype):
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda:
         raise TypeError(f"{what} expects a 2-D CUDA tensor")
     T, H = x.shape
+    if T > _MOST_ROWS:  # a larger number would not arrive whole
+        raise RuntimeError(f"{what} takes at most 2^30 rows, got {T}")
     dev = x.device
     xt = dtype_code(x.dtype)
     _no_grad(what, x, residual, weight)

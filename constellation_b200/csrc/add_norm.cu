@@ -348,8 +348,8 @@ extern "C" int cst_add_rmsnorm(const void* x, int32_t x_dtype, int64_t ld_x, con
     if (!act(x_dtype) || (residual && !act(residual_dtype)) || !(act(out_dtype) || out_dtype == CST_DTYPE_E4M3))
         return set_last_error(CST_ERR_INVALID_ARG, "invalid dtype (x %d, residual %d, out %d)", x_dtype,
                               residual_dtype, out_dtype);
-    if (T < 0 || H < 1 || H > kMaxNormWidth)
-        return set_last_error(CST_ERR_INVALID_ARG, "T=%d must be >= 0 and H=%d in [1, %d]", T, H, kMaxNormWidth);
+    if (T < 0 || T > (1 << 30) || H < 1 || H > kMaxNormWidth)
+        return set_last_error(CST_ERR_INVALID_ARG, "T=%d must be in [0, 2^30] and H=%d in [1, %d]", T, H, kMaxNormWidth);
     if (ld_x < H || ld_out < H || (residual && ld_residual < H) || (residual && sum && ld_sum < H))
         return set_last_error(CST_ERR_INVALID_ARG, "a row stride is below H=%d", H);
     if (!residual && sum)

@@ -613,8 +613,8 @@ extern "C" int cst_unsort_rows(const void* rows, int32_t rows_dtype, int64_t ld_
     if (!act_dtype(rows_dtype) || !act_dtype(out_dtype) || (residual && !act_dtype(residual_dtype)))
         return set_last_error(CST_ERR_INVALID_ARG, "invalid dtype (rows %d, residual %d, out %d)", rows_dtype,
                               residual_dtype, out_dtype);
-    if (H < 1 || ld_rows < H || (residual && ld_residual < H))
-        return set_last_error(CST_ERR_INVALID_ARG, "H=%d must be positive and no row stride below it", H);
+    if (H < 1 || H > (1 << 30) || ld_rows < H || (residual && ld_residual < H))
+        return set_last_error(CST_ERR_INVALID_ARG, "H=%d must be in [1, 2^30] and no row stride below it", H);
     if (T == 0) return CST_OK;
     if (!rows || !row_of || !out) return set_last_error(CST_ERR_INVALID_ARG, "null rows, order or out");
     const UnsortArgs a{rows, rows_dtype, ld_rows, row_of, weight, T, K, H, residual, residual_dtype, ld_residual, out,
@@ -641,8 +641,8 @@ extern "C" int cst_unsort_rows_grad(const void* grad, int32_t grad_dtype, int64_
     if (const int rc = check_routes("unsort_rows_grad", T, K)) return rc;
     if (!act_dtype(grad_dtype) || !act_dtype(rows_dtype))
         return set_last_error(CST_ERR_INVALID_ARG, "invalid dtype (grad %d, rows %d)", grad_dtype, rows_dtype);
-    if (H < 1 || ld_grad < H || (d_weight && ld_rows < H))
-        return set_last_error(CST_ERR_INVALID_ARG, "H=%d must be positive and no row stride below it", H);
+    if (H < 1 || H > (1 << 30) || ld_grad < H || (d_weight && ld_rows < H))
+        return set_last_error(CST_ERR_INVALID_ARG, "H=%d must be in [1, 2^30] and no row stride below it", H);
     if (T == 0 || (!d_rows && !d_weight)) return CST_OK;
     if (!grad || !row_of || !rows_used || (d_weight && !rows))
         return set_last_error(CST_ERR_INVALID_ARG, "null grad, rows or order");

@@ -145,8 +145,8 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     if dev != w.device:
         raise RuntimeError(f"device mismatch: x={dev} weight={w.device}")
     R, K = x.shape
-    if K != w.k:
-        raise RuntimeError(f"x must be [R, {w.k}], got {tuple(x.shape)}")
+    if K != w.k or R > 1 << 28:
+        raise RuntimeError(f"x must be [R, {w.k}] with R at most 2^28, got {tuple(x.shape)}")
     if x.dtype == torch.float8_e4m3fn:
         xt = CST_DTYPE_E4M3
         if x_scale is None:

@@ -26,7 +26,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check
-from .context import _empty, _on, _ptr, _rows, _stream, dtype_code
+from .context import _MOST_ROWS, _empty, _on, _ptr, _rows, _stream, dtype_code
 
 
 @dataclass(frozen=True)
@@ -39,7 +39,8 @@ class TokenOrder:
 
     def __post_init__(self):
         r, q, o = self.row_of, self.route_of, self.offsets
-        if r.dim() != 2 or q.dim() != 1 or o.dim() != 1 or q.shape[0] != r.numel() or o.shape[0] < 2:
+        if r.dim() != 2 or q.dim() != 1 or o.dim() != 1 or q.shape[0] != r.numel() or o.shape[0] < 2 \
+                or q.shape[0] > _MOST_ROWS:
             raise RuntimeError("not an order: row_of [T, K], route_of [T * K] and offsets [n_experts + 1] are expected")
         dev = r.device
         for t in (r, q, o):
@@ -57,11 +58,15 @@ def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0
         raise TypeError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
     T, K = topk_idx.shape
     n = T * K
+    if n > _MOST_ROWS:
+        raise RuntimeError(f"sort_routes takes at most 2^30 routes, got {n}")
     dev = topk_idx.device
     topk_idx = topk_idx.contiguous()
     n_experts = int(n_experts)
     if not 1 <= n_experts <= 1024:
         raise ValueError(f"n_experts must be in [1, 1024], got {n_experts}")
+    if not 0 <= first_expert < 1 << 31:
+        raise ValueError(f"first_expert must be in [0, 2^31), got {first_expert}")
     row_of = _empty(T, K, torch.int32, dev)
     route_of = torch.empty_strided((n,), (1,), dtype=torch.int32, device=dev)
     offsets = torch.empty_strided((n_experts + 1,), (1,), dtype=torch.int32, device=dev)
@@ -80,8 +85,8 @@ def _check_order(order: TokenOrder, dev: torch.device) -> None:
 def _matrix(name: str, t: torch.Tensor, rows: int) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_cuda:
         raise TypeError(f"{name} must be a 2-D CUDA tensor")
-    if t.shape[0] != rows or t.shape[1] < 1:
-        raise RuntimeError(f"{name} must be [{rows}, H >= 1], got {tuple(t.shape)}")
+    if t.shape[0] != rows or not 1 <= t.shape[1] <= 1 << 30:
+        raise RuntimeError(f"{name} must be [{rows}, H] with H in [1, 2^30], got {tuple(t.shape)}")
 
 
 def _wants_grad(*tensors) -> bool:

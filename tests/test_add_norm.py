@@ -257,7 +257,8 @@ def test_refusals_of_device_tensors():
            lambda: add_rms_norm(x, res, w, sum_out=torch.empty(4, 256, device="cuda")),
            lambda: add_rms_norm(x, res, w, out=torch.empty(256, 4, device="cuda").t()),
            lambda: add_rms_norm(x, res, w, out=torch.empty(1, 256, device="cuda").expand(4, 256)),
-           lambda: add_rms_norm_fp8(x, None, w, sum_out=res), lambda: add_rms_norm(x.float().requires_grad_(), res, w)]
+           lambda: add_rms_norm_fp8(x, None, w, sum_out=res), lambda: add_rms_norm(x.float().requires_grad_(), res, w),
+           lambda: add_rms_norm_fp8(x[:1, :1].expand(2 ** 32 + 1, 1))]
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
@@ -285,7 +286,7 @@ def test_refusals_without_a_device():
         return L.cst_add_rmsnorm(x, xt, ldx, res, rt, ldr, T, H, None, 1e-6, sum_, lds, out, ot, ldo, scale, None)
 
     assert call(x=None, res=None, out=None, T=0) == _lib.CST_OK
-    for kw in (dict(xt=4), dict(rt=0), dict(ot=5), dict(H=0), dict(H=32769), dict(T=-1), dict(ldx=255), dict(ldr=1),
+    for kw in (dict(xt=4), dict(rt=0), dict(ot=5), dict(H=0), dict(H=32769), dict(T=-1), dict(T=2 ** 30 + 1), dict(ldx=255), dict(ldr=1),
                dict(ldo=255), dict(sum_=P, lds=8), dict(x=None), dict(out=None), dict(ot=4), dict(res=None, sum_=P)):
         assert call(**kw) == _lib.CST_ERR_INVALID_ARG, kw
         assert _lib.last_error()

@@ -6,8 +6,8 @@ the next, so the error is that of the sums: at most one unit of 2^-23 of the sum
 group and a tree over parts of k: (group + 2 K / group + 64) * 2^-23 of sum |W x|.  Where zero points leave
 little of a group, its magnitude is that of scale (q + zero) |x|, and `check` is given those weights as `mag`.
 x itself is kept exactly down to 2^-13 (bf16) or 2^-11 (fp16) of its row's largest; what a smaller one loses
-is below 2^-21 (2^-22) of that largest, `drop`, which counts where a row has outliers: rows of randn hold no |x| above 6,
-so that drop * 6 * sum |W| is below 2^-18 sum |W|, a hundredth of the first term for their mean |x| of 0.8.
+is below 2^-21 (2^-22) of that largest, `drop`, which counts where a row has outliers: rows of randn hold no |x|
+above 6, so that drop * 6 * sum |W| is below 2^-18 sum |W|, a hundredth of the first term for their mean |x| of 0.8.
 The result is rounded once, eps(t) / 2 of the value.  silu has a slope below 1.1 and costs 8 * 2^-24 of its
 value.
 """
@@ -512,6 +512,7 @@ def test_refusals_of_device_tensors():
            lambda: grouped_int4(x, w, off, out=torch.empty(4, 63, device="cuda")),
            lambda: grouped_int4(x, w, off, out=torch.empty(4, 64, device="cuda"), out_dtype=torch.bfloat16),
            lambda: grouped_int4(x, w, off, out=x.view(-1)[:256].view(4, 64)),
+           lambda: grouped_int4(x[:1].expand(2 ** 32 + 4, 256), w, off),
            lambda: grouped_int4(x.clone().requires_grad_(), w, off)]
     for f in bad:
         with pytest.raises(RuntimeError):

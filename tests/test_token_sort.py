@@ -297,7 +297,8 @@ def test_refusals_of_device_tensors():
            lambda: sort_tokens(x, TokenOrder(o.row_of.long(), o.route_of, o.offsets)),
            lambda: sort_tokens(x, TokenOrder(o.row_of, o.route_of[:-1], o.offsets)),
            lambda: sort_tokens(x, TokenOrder(o.row_of.cpu(), o.route_of, o.offsets)),
-           lambda: sort_tokens(x.float().requires_grad_(), o, scale=w)]
+           lambda: sort_tokens(x.float().requires_grad_(), o, scale=w),
+           lambda: sort_routes(idx[:1, :1].expand(2 ** 32 + 1, 1), E)]
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
@@ -306,9 +307,9 @@ def test_refusals_of_device_tensors():
               lambda: unsort_tokens(rows, o, w, out_dtype=torch.float64)):
         with pytest.raises(TypeError):
             f()
-    for n in (0, 1025):
+    for n, first in ((0, 0), (1025, 0), (E, -1), (E, 2 ** 32)):
         with pytest.raises(ValueError):
-            sort_routes(idx, n)
+            sort_routes(idx, n, first_expert=first)
 
 
 @gpu
@@ -353,8 +354,8 @@ def test_refusals_without_a_device(monkeypatch):
     un = lambda r=P, dt=2, ld=64, T=1, K=1, H=64, res=None, rt=2, ldr=64, out=P, ot=2: L.cst_unsort_rows(  # noqa: E731
         r, dt, ld, P, None, T, K, H, res, rt, ldr, out, ot, None)
     assert un(r=None, T=0, out=None) == _lib.CST_OK
-    for kw in (dict(dt=4), dict(ot=0), dict(res=P, rt=9), dict(ld=63), dict(H=0), dict(res=P, ldr=1), dict(r=None),
-               dict(out=None), dict(K=2000)):
+    for kw in (dict(dt=4), dict(ot=0), dict(res=P, rt=9), dict(ld=63), dict(H=0), dict(H=2 ** 30 + 1, ld=2 ** 40),
+               dict(res=P, ldr=1), dict(r=None), dict(out=None), dict(K=2000)):
         assert un(**kw) == BAD, kw
     gr = lambda g=P, gt=2, ldg=64, r=P, dt=2, ld=64, T=1, H=64, dr=P, dw=P: L.cst_unsort_rows_grad(  # noqa: E731
         g, gt, ldg, r, dt, ld, P, P, P, T, 1, H, dr, dw, None)
