@@ -48,6 +48,13 @@ class TokenOrder:
                 raise RuntimeError("an order is contiguous int32 on one device")
 
 
+def _made(row_of, route_of, offsets) -> TokenOrder:
+    """A ``TokenOrder`` of tensors that were made as one, without the checks of one that a caller makes."""
+    order = object.__new__(TokenOrder)
+    order.__dict__.update(row_of=row_of, route_of=route_of, offsets=offsets)
+    return order
+
+
 def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0) -> TokenOrder:
     """The order of ``topk_idx`` (``[T, K]`` int32 or int64) over the experts ``[first_expert,
     first_expert + n_experts)``, at most 1024; any other id, -1 among them, is a route to an expert
@@ -74,7 +81,7 @@ def sort_routes(topk_idx: torch.Tensor, n_experts: int, *, first_expert: int = 0
         check(_lib.lib.cst_sort_routes(topk_idx.data_ptr(), topk_idx.element_size(), T, K, n_experts,
                                        int(first_expert), row_of.data_ptr(), route_of.data_ptr(), offsets.data_ptr(),
                                        _stream(dev)))
-    return TokenOrder(row_of, route_of, offsets)
+    return _made(row_of, route_of, offsets)
 
 
 def _check_order(order: TokenOrder, dev: torch.device) -> None:
@@ -148,7 +155,7 @@ class _SortTokens(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         _refuse_capture("sort_tokens")
-        return sort_tokens_backward(grad, TokenOrder(*ctx.saved_tensors)), None
+        return sort_tokens_backward(grad, _made(*ctx.saved_tensors)), None
 
 
 class _UnsortTokens(torch.autograd.Function):
@@ -168,7 +175,7 @@ class _UnsortTokens(torch.autograd.Function):
     def backward(ctx, grad):
         _refuse_capture("unsort_tokens")
         saved = ctx.saved_tensors
-        order = TokenOrder(*saved[:3])
+        order = _made(*saved[:3])
         weight = saved[3] if ctx.weighted else None
         rows = saved[4] if ctx.has_rows else None
         d_rows, d_weight = _unsort_grad(grad, rows, ctx.rows_dtype, order, weight, ctx.needs_input_grad[0],
