@@ -91,6 +91,7 @@ struct Around {
     uint4 lo, hi;
     uint32_t off;
     __device__ __forceinline__ uint4 piece() const {
+        if (off == 0) return lo;  // mostly of a whole warp
         const bool two = off & 8u, one = off & 4u;
         const uint32_t a0 = two ? lo.z : lo.x, a1 = two ? lo.w : lo.y, a2 = two ? hi.x : lo.z, a3 = two ? hi.y : lo.w,
                        a4 = two ? hi.z : hi.x, a5 = two ? hi.w : hi.y;

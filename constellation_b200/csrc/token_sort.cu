@@ -293,8 +293,9 @@ struct UnsortArgs {
 // A thread takes 8 columns of a token and loads them of up to 8 of its rows before it adds any, so a sum costs
 // one wait for memory.  DT: the rows' type where it is 16 bits, 0 otherwise.  Vectors are numbered through
 // all tokens, so that narrow rows fill a CTA.  Bound by HBM: 4096 tokens of 8 rows of 7168 bf16 111 us (5.3 TB/s),
-// 64 tokens 3.2 us.  ANY is bound by the shifting of what lies across 16 bytes: 2048 tokens of 5001 columns 91 us
-// (2.3 TB/s); with all 8 rows loaded ahead it needed 111 registers and took 97 us.
+// 64 tokens 3.2 us.  ANY is bound by the shifting of what lies across 16 bytes: 2048 tokens of 5001 columns 69 us
+// (3.0 TB/s; 91 us when pieces on a boundary were shifted too).  With all 8 rows loaded ahead it needed 111 registers
+// and was slower.
 template <int DT, bool ANY>
 __global__ void __launch_bounds__(256) unsort_kernel(UnsortArgs a, int vectors) {
     constexpr int kAhead = 8;
@@ -375,7 +376,7 @@ struct UnsortGradArgs {
 // One CTA a token, kAhead of its routes at a time: a thread loads 8 columns of the gradient and of these routes'
 // rows together, stores the rows' gradients and keeps a partial dot product for each.  DT: the type of g, rows and
 // d_rows where all have it, 0 otherwise.  Bound by HBM: 4096 tokens of 8 rows of 7168 bf16 184 us (5.4 TB/s).  ANY:
-// 2048 tokens of 5001 columns 142 us (2.5 TB/s; 184 us with one route after the other).
+// 2048 tokens of 5001 columns 146 us (2.4 TB/s; 184 us with one route after the other).
 template <int DT, bool ANY>
 __global__ void __launch_bounds__(256) unsort_grad_kernel(UnsortGradArgs a) {
     constexpr int kAhead = 8;
