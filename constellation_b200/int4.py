@@ -95,6 +95,7 @@ class Int4Weight:
 
     def _pack(self, first, count, q, scale, zero):
         G = self.k // self.group
+        _no_grad("Int4Weight", scale)
         if (zero is not None) != self.zero_points:
             raise RuntimeError("zero points are given for all experts of a weight or for none")
         for name, t, shape, dtype in (("q", q, (count, self.n, self.k // 2), torch.uint8),
@@ -160,7 +161,7 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
             raise RuntimeError("x_scale goes with e4m3 rows")
     else:
         raise TypeError(f"x must be float16, bfloat16 or float8_e4m3fn, got {x.dtype}")
-    _no_grad("grouped_int4", x)
+    _no_grad("grouped_int4", x, x_scale)
     if offsets is None:
         if w.n_experts != 1:
             raise RuntimeError(f"offsets are needed for {w.n_experts} experts")

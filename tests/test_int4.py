@@ -513,7 +513,9 @@ def test_refusals_of_device_tensors():
            lambda: grouped_int4(x, w, off, out=torch.empty(4, 64, device="cuda"), out_dtype=torch.bfloat16),
            lambda: grouped_int4(x, w, off, out=x.view(-1)[:256].view(4, 64)),
            lambda: grouped_int4(x[:1].expand(2 ** 32 + 4, 256), w, off),
-           lambda: grouped_int4(x.clone().requires_grad_(), w, off)]
+           lambda: grouped_int4(x.clone().requires_grad_(), w, off),
+           lambda: grouped_int4(x8, w, off, x_scale=xs.clone().requires_grad_()),
+           lambda: Int4Weight(q, s.clone().requires_grad_(), z)]
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
