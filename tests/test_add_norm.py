@@ -132,7 +132,7 @@ def test_strides_and_offsets(H, offset, stride):
 @gpu
 @pytest.mark.parametrize("T,H,offset,stride", [(640, 8, 0, 8), (640, 250, 0, 256), (700, 256, 8, 272), (1300, 2048, 0, 2048),
                                                (640, 8192, 0, 8192), (640, 5001, 1, 5003), (3, 9001, 1, 9003),
-                                               (640, 9001, 0, 9001), (700, 8200, 0, 8200)])
+                                               (640, 9001, 0, 9001), (700, 8200, 0, 8200), (301, 16384, 8, 16400)])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 def test_many_rows(T, H, offset, stride, dt):
     """Long batches go from row to row: a row's numbers reach no other row, with and without what is optional."""
