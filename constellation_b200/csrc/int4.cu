@@ -774,6 +774,9 @@ __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s
     uint32_t turn = 0;
     if (lane == 0 && set == 0)  // no accumulators to take before the first products
         for (int j = 0; j < a.bufs; ++j) mbar_arrive(&sh.ready[j]);
+    // The rows' scales are split_x_kernel's.  A CTA whose cluster has more CTAs than its items have steps of k waits for
+    // no product before it reads them.
+    if constexpr (TERMS > 1) chain_wait();
     for (int64_t i = sp.first; i < sp.items; i += sp.step, ++turn) {
         const Item it = find_item(a, sh.tile, sh.row, i);
         float* part = s_part + (a.ranks > 1 ? (turn & 1) * kSets * size : 0);  // [set][row of x][weight row]
@@ -787,7 +790,7 @@ __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s
         if (it.rows <= 8) item(std::integral_constant<int, 8>{});
         else if (it.rows <= 16) item(std::integral_constant<int, 16>{});
         else item(std::integral_constant<int, 32>{});
-        // Lane t has the scale of row t.  (The products above have read x's terms, so it is written.)
+        // Lane t has the scale of row t.
         const float scale = TERMS > 1 && lane < it.rows ? __ldcg(a.facts + it.row + lane) : 1.0f;
         int t0 = 0, t1 = it.rows;
         output_sync();
@@ -852,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
     if (a.ranks > 1) cluster_barrier();  // every CTA's barriers exist before any CTA arrives on them
     // The kernel before this one on the stream is split_x_kernel, which let this one start only after it had
     // waited for everything before it: offsets and weights are there, and `out` is free.  What it writes
-    // itself, x's terms and facts, only the producer reads, after its own wait.
+    // itself, x's terms and facts, the producer and the output warps read, each after a wait of its own.
     chain_release();
     scan_offsets(a, sh.tile, sh.row, sh.scan);
 
