@@ -295,7 +295,7 @@ class Int4Experts:
         if not 0 <= b <= e <= x.shape[0]:
             raise RuntimeError(f"invalid shared range [{b}, {e}) of {x.shape[0]} tokens")
         extra = None
-        if self._shared is not None and e > b:
+        if e > b:
             extra = self._shared_rows(x[b:e])
             if e - b < x.shape[0]:
                 whole = torch.zeros((x.shape[0], extra.shape[1]), dtype=torch.float32, device=self.device)
