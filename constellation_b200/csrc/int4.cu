@@ -562,8 +562,9 @@ __device__ __forceinline__ void widen_role(const Int4Args& a, Shared& sh, const 
     const int quarter = (int(threadIdx.x) >> 5) & 3;  // the lanes of tensor memory this warp may touch
     const int row = quarter * 32 + lane;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    if (!a.g.has_zero) {  // -8 * 2^-9 for every product of this launch; the first arrival below orders it
-        if (set == 0) tmem_fill8(lanes + a.z_at, 0x88888888u);
+    if (!a.g.has_zero && set == 0) {  // -8 * 2^-9 for every product of this launch; the first arrival below orders it
+        tmem_fill8(lanes + a.z_at, 0x88888888u);
+        tmem_wait_st();  // here, for a CTA without items has no step that waits, and gives its columns back
     }
     Ring s, b;
     int turn = set;

@@ -56,3 +56,24 @@ def test_row_scales_of_a_split_k(R, N, K, group, zeros, dt):
     for byte in (0xFF, 0x47, 0xFF):  # NaN, then scales of 5e4, in the scales' place
         room.fill_(byte)
         check(product_in(room, x, w, None), x.double(), W, None, group, False)
+
+
+@gpu
+def test_ctas_without_products_between_products():
+    """A grid is sized for rows of every expert: with all rows at one expert most CTAs find no item, with none at any all
+    do, and they give their tensor memory back to the products that follow."""
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    E, N, K, R = 64, 256, 384, 48
+    weights = [make_weight(E, N, K, 128, zeros) for zeros in (False, True)]
+    held = [Int4Weight(q, s, z) for q, s, z, _ in weights]
+    x, _, x64 = make_x(R, K, torch.bfloat16)
+    ragged = [R * e // E for e in range(E + 1)]
+    orders = [torch.tensor(off, dtype=torch.int32, device="cuda")
+              for off in ([0] * 7 + [R] * (E - 6), [0] * (E + 1), ragged)]
+    got = [(i, off, grouped_int4(x, held[i], off, out_dtype=torch.float32))
+           for _ in range(8) for off in orders for i in range(2)]
+    for i, off, out in got:
+        check(out, x64, weights[i][3], off, 128, False)
+    for w in held:
+        w.device_error()
