@@ -1036,6 +1036,23 @@ int check_x_dtype(int x_dtype) {
     return CST_OK;
 }
 
+// Rows in memory: `rows` of `bytes`, `pitch` bytes apart.
+struct Extent {
+    const void* p;
+    int64_t rows, bytes, pitch;
+    uint64_t first() const { return reinterpret_cast<uintptr_t>(p); }
+    uint64_t end() const { return first() + uint64_t((rows - 1) * pitch + bytes); }
+};
+
+// Whether two extents may share a byte; columns of one array that lie side by side share none.
+bool overlap(const Extent& a, const Extent& b) {
+    if (!a.p || !b.p || a.first() >= b.end() || b.first() >= a.end()) return false;
+    if (a.pitch != b.pitch) return true;
+    const int64_t shift = b.first() >= a.first() ? int64_t((b.first() - a.first()) % uint64_t(a.pitch))
+                                                 : a.pitch - 1 - int64_t((a.first() - b.first() - 1) % uint64_t(a.pitch));
+    return shift < a.bytes || shift + b.bytes > a.pitch;
+}
+
 int check_weight(const cst_int4_weight* w) {
     if (!w) return set_last_error(CST_ERR_INVALID_ARG, "null weight");
     if (w->n_experts < 1 || w->n_experts > CST_INT4_MAX_EXPERTS || w->n < 1 || w->k < 1 || w->n > (1 << 20) ||
@@ -1134,6 +1151,25 @@ extern "C" int cst_grouped_int4(const cst_int4_weight* w, void* data, const void
         return set_last_error(CST_ERR_INVALID_ARG, "null data, x, workspace or out");
     if (((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(workspace)) & 15u))
         return set_last_error(CST_ERR_INVALID_ARG, "data and workspace must be 16-byte aligned");
+    // Rows of `out` are written before the last of these is read: by the product's CTAs while others have not begun,
+    // and where they belong to no expert even beside split_x_kernel.
+    const int64_t x_size = act_size(x_dtype), out_size = act_size(out_dtype), xs = (w->k + kChunk - 1) / kChunk;
+    const Extent written{out, R, g.out_n * out_size, ld_out * out_size};
+    int64_t data_bytes = 0, room_bytes = 0;
+    cst_int4_bytes(w, &data_bytes);
+    cst_int4_workspace(w, x_dtype, R, &room_bytes);
+    const struct {
+        const char* name;
+        Extent at;
+    } read[] = {{"x", {x, R, w->k * x_size, ld_x * x_size}},
+                {"x_scale", {x_scale, R, xs * 4, ld_x_scale * 4}},
+                {"offsets", {offsets, 1, (w->n_experts + 1) * 4, (w->n_experts + 1) * 4}},
+                {"the weight", {data, 1, data_bytes, data_bytes}},
+                {"the workspace", {workspace, 1, room_bytes, room_bytes}}};
+    for (const auto& r : read)
+        if (overlap(written, r.at))
+            return set_last_error(CST_ERR_INVALID_ARG, "out overlaps %s, which is still read while results are written",
+                                  r.name);
     const int sms = current_sms();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Int4Args a{};

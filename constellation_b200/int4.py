@@ -135,7 +135,7 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     leaves them, sorted by ``sort_tokens``).  ``offsets`` is int32 ``[E + 1]`` on the device, ascending
     (``TokenOrder.offsets``); without it there is one weight and it takes every row.  The result is
     ``[R, N]`` (``[R, N / 2]`` with swiglu) in ``out_dtype``: fp16, bf16 or fp32; by default ``x``'s type, bf16
-    for e4m3 rows.  ``out`` may not overlap ``x``.
+    for e4m3 rows.  ``out`` may not overlap ``x``, ``x_scale``, ``offsets`` or the weight's ``data``.
 
     fp32 sums, one rounding.  fp16 and bf16 rows enter as 8-bit terms: exactly where a number is above 2^-11 (fp16)
     or 2^-13 (bf16) of its row's largest, and with an error below 2^-22 (2^-21) of that largest elsewhere.  So a row
@@ -174,10 +174,6 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     elif (out.shape != (R, w.out_features) or out.device != dev or not out.is_contiguous()
           or out_dtype not in (None, out.dtype)):
         raise RuntimeError(f"out must be contiguous [{R}, {w.out_features}] on the device of x, of the out_dtype given")
-    elif R and x.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
-        first, last = x.data_ptr(), x.data_ptr() + ((R - 1) * x.stride(0) + K) * x.element_size()
-        if out.data_ptr() < last and first < out.data_ptr() + out.numel() * out.element_size():
-            raise RuntimeError("out overlaps x, whose rows are still read while results are written")
     ot = dtype_code(out.dtype)
     x, ldx = _rows(x)
     lds = 0

@@ -330,6 +330,8 @@ int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int32_t R, int
  *   x    [R, k] fp16, bf16, or e4m3 with x_scale [R, ceil(k / 128)] fp32 (NULL otherwise)
  *   workspace  cst_int4_workspace bytes, 16-byte aligned, of this call alone until it is done
  *   out  [R, n] (n / 2 with swiglu) in out_dtype (fp16, bf16, fp32)
+ * `out` may not overlap x, x_scale, offsets, data or workspace, which are read while it is written
+ * (CST_ERR_INVALID_ARG); it may be other columns of x's array, at the same row pitch in bytes.
  * x enters the products as 8-bit terms that hold it exactly but for what is below 2^-21 (bf16) or
  * 2^-22 (fp16) of the largest |x| of its row; sums are fp32, with one rounding.
  * An infinity in a row of x makes the row's results NaN.  `data` is only read, but for its error word. */

@@ -77,3 +77,70 @@ def test_ctas_without_products_between_products():
         check(out, x64, weights[i][3], off, 128, False)
     for w in held:
         w.device_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses stay on machines that could not launch a kernel")
+def test_an_out_that_overlaps_an_input_is_refused():
+    """By address alone, so nothing is read, written or launched; what is refused lies at made-up addresses."""
+    import ctypes
+
+    from constellation_b200 import _lib
+
+    L, BAD, MB = _lib.lib, _lib.CST_ERR_INVALID_ARG, 1 << 20
+    w = ctypes.byref(_lib.CstInt4Weight(2, 64, 256, 128, 1, 0, 0))
+    size = ctypes.c_int64()
+    assert L.cst_int4_bytes(w, ctypes.byref(size)) == 0
+    data = size.value
+    assert L.cst_int4_workspace(w, 4, 8, ctypes.byref(size)) == 0
+    room = size.value
+
+    def call(out, ldo=64, ot=2, xt=4, ldx=256, lds=2):
+        xs = 2 * MB if xt == 4 else None
+        rc = L.cst_grouped_int4(w, 4 * MB, MB, xt, ldx, xs, lds, 3 * MB, 8, 5 * MB, out, ot, ldo, None)
+        return rc == BAD and b"overlaps" in L.cst_last_error()
+
+    # out takes 8 * 64 * 2 bytes
+    for first, last in ((MB, MB + 8 * 256), (2 * MB, 2 * MB + 8 * 2 * 4), (3 * MB, 3 * MB + 3 * 4),
+                        (4 * MB, 4 * MB + data), (5 * MB, 5 * MB + room)):
+        for out in (first - 1024 + 2, first, last - 2):
+            assert call(out)
+    assert call(MB + 300, ldx=512)  # from the gap behind a row on, at another pitch
+    # columns of one array of 1024 bytes a row: x (bf16, 512 bytes) at 0 (and one where rows wrap into it)
+    for out in (MB + 510, MB - 1024 + 900, MB + 1024 * 7 + 510):
+        assert call(out, ldo=512, xt=2, ldx=512)
+
+
+@gpu
+def test_out_beside_the_inputs():
+    """Next to its inputs in one buffer an out is taken, on top of any of them it is not."""
+    from constellation_b200 import _lib
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    q, s, z, W = make_weight(2, 64, 256, 128, False)
+    w, off = Int4Weight(q, s), offsets_of((3, 4))
+    x, xs, x64 = make_x(8, 256, torch.float8_e4m3fn)
+    want = grouped_int4(x, w, off, x_scale=xs)
+    buf = torch.zeros(16384, dtype=torch.uint8, device="cuda")
+
+    def put(at, t):
+        buf[at:at + t.numel() * t.element_size()] = t.contiguous().view(torch.uint8).view(-1)
+        return buf[at:at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+
+    # x 2048 bytes, its scales 64, offsets 12, out 1024
+    x1, xs1, off1 = put(1024, x), put(3072, xs), put(3136, off)
+    for at in (0, 3152):
+        out = buf[at:at + 1024].view(torch.bfloat16).view(8, 64)
+        assert torch.equal(grouped_int4(x1, w, off1, x_scale=xs1, out=out), want)
+    for at in (16, 1024, 2048, 3056, 3120, 3136):
+        out = buf[at:at + 1024].view(torch.bfloat16).view(8, 64)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            grouped_int4(x1, w, off1, x_scale=xs1, out=out)
+    # other columns of x's array
+    xb, _, xb64 = make_x(8, 256, torch.bfloat16)
+    wide = torch.zeros(8, 320, dtype=torch.bfloat16, device="cuda")
+    wide[:, :256] = xb
+    room = torch.empty(w._workspace(2, 8), dtype=torch.uint8, device="cuda")
+    _lib.check(_lib.lib.cst_grouped_int4(w._ref, w.data.data_ptr(), wide.data_ptr(), 2, 320, None, 0, off.data_ptr(), 8,
+                                         room.data_ptr(), wide.data_ptr() + 512, 2, 320,
+                                         torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(wide[:, 256:], grouped_int4(xb, w, off)) and torch.equal(wide[:, :256], xb)
