@@ -14,6 +14,7 @@ import ctypes
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import CST_DTYPE_BF16, CST_DTYPE_E4M3, CST_DTYPE_FP16, CST_DTYPE_FP32, check
@@ -109,10 +110,19 @@ def _on(device: torch.device):
     return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _no_tangent(what: str, *tensors) -> None:
+    """Refuse dual tensors of forward-mode differentiation, whose tangents an operator would drop silently."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual tensor lives; asking each costs 0.4 us
+        return
+    if any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise RuntimeError(f"{what} has no forward-mode derivative; call it on detached tensors")
+
+
 def _no_grad(what: str, *tensors) -> None:
     """Refuse inputs whose gradient an operator without a backward pass would drop silently."""
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
         raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad() or on detached tensors")
+    _no_tangent(what, *tensors)
 
 
 def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:

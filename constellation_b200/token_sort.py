@@ -14,8 +14,9 @@ Shapes depend on ``T`` and ``K`` alone: routes to experts held elsewhere leave r
 results repeat bit for bit.
 
 ``sort_tokens`` and ``unsort_tokens`` record their gradients where an input asks for one (not twice
-differentiable).  Under CUDA graph capture autograd is refused, on both passes: a capture calls
-``sort_tokens_backward`` and ``unsort_tokens_backward``, which are plain launches.
+differentiable; forward-mode tangents are refused).  Under CUDA graph capture autograd is refused, on
+both passes: a capture calls ``sort_tokens_backward`` and ``unsort_tokens_backward``, which are plain
+launches.
 """
 from __future__ import annotations
 
@@ -26,7 +27,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check
-from .context import _MOST_ROWS, _empty, _on, _ptr, _rows, _stream, dtype_code
+from .context import _MOST_ROWS, _empty, _no_tangent, _on, _ptr, _rows, _stream, dtype_code
 
 
 @dataclass(frozen=True)
@@ -174,6 +175,7 @@ class _UnsortTokens(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         _refuse_capture("unsort_tokens")
+        _no_tangent("unsort_tokens' gradient", grad)
         saved = ctx.saved_tensors
         order = _made(*saved[:3])
         weight = saved[3] if ctx.weighted else None
@@ -195,6 +197,7 @@ def sort_tokens(x: torch.Tensor, order: TokenOrder, *, scale: torch.Tensor | Non
     _check_order(order, x.device)
     if x.dtype != torch.float8_e4m3fn:
         dtype_code(x.dtype)
+    _no_tangent("sort_tokens", x, scale)
     if scale is not None:
         _matrix("scale", scale, T)
         if scale.dtype != torch.float32 or scale.device != x.device:
@@ -233,6 +236,7 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, weight: torch.Tensor | 
         dtype_code(residual.dtype)
         if residual.shape[1] != rows.shape[1] or residual.device != rows.device:
             raise RuntimeError("residual must be [T, H] on the device of rows")
+    _no_tangent("unsort_tokens", rows, weight, residual)
     if _wants_grad(rows, weight, residual):
         _refuse_capture("unsort_tokens")
         return _UnsortTokens.apply(rows, weight, residual, order, out_dtype)
@@ -244,6 +248,7 @@ def sort_tokens_backward(grad_rows: torch.Tensor, order: TokenOrder) -> torch.Te
     T, K = order.row_of.shape
     _matrix("grad_rows", grad_rows, T * K)
     _check_order(order, grad_rows.device)
+    _no_tangent("sort_tokens_backward", grad_rows)
     return _unsort(grad_rows.detach(), order, None, None, grad_rows.dtype)
 
 
@@ -261,6 +266,8 @@ def unsort_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, order: TokenO
     if weight is not None:
         if weight.dtype != torch.float32 or weight.shape != (T, K) or weight.device != rows.device:
             raise RuntimeError(f"weight must be fp32 [{T}, {K}] on the device of rows")
+    _no_tangent("unsort_tokens_backward", grad, rows, weight)
+    if weight is not None:
         weight = weight.detach().contiguous()
     return _unsort_grad(grad.detach(), rows.detach(), rows.dtype, order, weight, True, weight is not None)
 
