@@ -113,19 +113,29 @@ def plan_dispatch(topk_idx: torch.Tensor, experts_per_rank: int, world: int) -> 
     return DispatchPlan(order=order, dest=dest, counts=counts, inv=inv.reshape(Tl, K))
 
 
+#: what each exchange calls of its compute object
+_CALLS = {"allgather": ("route", "moe_routed_range", "cast_extra"),
+          "alltoall": ("route", "find_slot", "find_shared_slot", "grouped_ffn", "combine_rows"),
+          "p2p": ("route", "moe_routed_push", "reduce_pushed")}
+
+
 class ExpertParallelMoE:
     """One MoE layer sharded over ``world`` ranks.
 
     ``compute`` is the rank's ``ExpertContext`` holding its ``experts_per_rank`` routed
-    experts (router ids ``[rank * epr, (rank + 1) * epr)``) and the shared expert.
+    experts (router ids ``[rank * epr, (rank + 1) * epr)``) and the shared expert, or an object with the
+    calls that ``mode`` makes (``int4.Int4Experts``: the all-gather exchange).
     """
 
     def __init__(self, compute, *, rank: int, world: int, n_routed_experts: int, group=None,
                  mode: str = "allgather", local_route_min: int = 128, p2p_tl_cap: int | None = None):
         if n_routed_experts % world:
             raise ValueError(f"{n_routed_experts} experts do not shard over {world} ranks")
-        if mode not in ("allgather", "alltoall", "p2p"):
+        if mode not in _CALLS:
             raise ValueError(f"unknown EP mode {mode!r}")
+        missing = [name for name in _CALLS[mode] if not hasattr(compute, name)]
+        if world > 1 and missing:
+            raise ValueError(f"{type(compute).__name__} does not support EP mode {mode!r} (no {', '.join(missing)})")
         self.c = compute
         self.rank, self.world, self.group, self.mode = rank, world, group, mode
         self.E = n_routed_experts

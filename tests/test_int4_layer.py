@@ -34,3 +34,17 @@ def test_a_shared_expert_that_is_not_resident_is_an_error():
             ex.moe_routed_range(x, idx, weight, b, e)
     with pytest.raises(RuntimeError, match="no shared expert is resident"):
         ex.moe_routed(x, idx, weight, add_shared=True)
+
+
+def test_an_exchange_that_a_compute_object_does_not_know_is_refused_at_once():
+    from constellation_b200.ep import ExpertParallelMoE
+    from constellation_b200.stack import MoEStack, StackLayer
+
+    ex = experts_without_a_device()
+    for mode in ("p2p", "alltoall"):
+        with pytest.raises(ValueError, match="Int4Experts"):
+            ExpertParallelMoE(ex, rank=0, world=2, n_routed_experts=4, mode=mode)
+        with pytest.raises(ValueError, match=mode):
+            MoEStack([StackLayer(ex, None, None)], rank=1, world=2, n_routed_experts=4, mode=mode)
+        assert ExpertParallelMoE(ex, rank=0, world=1, n_routed_experts=4, mode=mode).c is ex  # nothing is exchanged
+    assert ExpertParallelMoE(ex, rank=1, world=2, n_routed_experts=4).c is ex
