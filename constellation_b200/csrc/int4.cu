@@ -12,7 +12,9 @@
 // into the same accumulator.  x enters as e4m3 terms with a power of two s that fits the largest |x| of the
 // row to 448: two terms for bf16 (8 bits = 4 + 4), x = s (t1 + t2 / 16), three for fp16 (11 bits),
 // x = s (t1 + t2 + t3 / 512).  They are x exactly where |x| is above 2^-13 (bf16) or 2^-11 (fp16) of that
-// largest; below, what they drop is less than 2^-21 (2^-22) of the largest.  e4m3 rows enter as they are,
+// largest; below, what they drop is less than 2^-21 (2^-22) of the largest.  A chunk of 128 columns whose own
+// largest lies 5 or more binades below the row's, as they do around an outlier, takes an s of its own, so what
+// it drops is at any rate less than 2^-17 (2^-18) of the chunk's largest.  e4m3 rows enter as they are,
 // with their scales.  The products are exact and the sums fp32, with one rounding at the end.
 //
 // Layout of one weight (written once by pack_kernel): blocks of 128 weight rows, each a run of
@@ -20,6 +22,7 @@
 // their zero points [128 / group][128].  q: [32 k][row][word of 8 k]; byte j of a word holds k = j in its
 // lower and k = 4 + j in its upper half.
 // With swiglu the rows of a block are 64 "up" rows, each followed by the "gate" row that goes with it.
+#include <cfloat>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -111,14 +114,24 @@ __global__ void __launch_bounds__(256) pack_kernel(Geom g, const uint8_t* q, con
 
 constexpr int kFactBytes = 16;  // of an e4m3 row and chunk: its scale, padded to what a bulk copy takes
 
+// A chunk whose largest lies within these binades of its row's takes the row's power of two.  Rows without outliers then
+// have one, which is multiplied once a result; powers of two of chunks are a load and a product for each accumulator.  A
+// launch with such rows took 16.5 us instead of 15.8 (8 rows of up and gate [4096, 7168]), 220 instead of 187 (64 experts of
+// 8 rows), 115 instead of 99 (254 fp16 rows of down [7168, 2048]) and 335 instead of 256 (groups of 32).
+constexpr int kNear = 4;
+
+// The exponent of a power of two for the terms of numbers up to `most`.
+__device__ __forceinline__ int terms_exp(float most) { return int(__float_as_uint(pow2_scale_for(most)) >> 23); }
+
 // One CTA a row.  terms: [rows * TERMS][chunks * 128] (of three terms [t1, t3, t2][rows][chunks * 128], so that one
-// product takes t1 and t3), columns past k zero.  facts: the rows' s; for e4m3
-// (TERMS 1) [chunks][rows] of x_scale, 16 bytes each.  A row's first 8192 columns stay in registers between
-// its maximum and its terms; more are read twice.
+// product takes t1 and t3), columns past k zero.  facts: [chunks][rows] of the power of two of a row's terms in a
+// chunk, negative in all of a row that has a chunk with one of its own; for e4m3 (TERMS 1) of x_scale, 16 bytes each.
+// A chunk is 8 columns of 16 threads, who find its largest by shuffles.  A row's first 8192 columns stay in registers
+// between its maximum and its terms; more are read twice.
 template <int TERMS>
 __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype, int64_t ld, const float* x_scale,
                                                       int64_t ld_xs, int rows, int k, uint8_t* terms, float* facts) {
-    __shared__ float s_most[8];
+    __shared__ float s_most[8], s_least[8];
     chain_wait();
     chain_release();
     const int chunks = (k + kChunk - 1) / kChunk, width = chunks * kChunk;
@@ -158,31 +171,57 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
         for (int j = 0; j < 8; ++j)
             if (isinf(v[j])) v[j] = __int_as_float(0x7fffffff);
     };
-    const int step = blockDim.x * 8, first = threadIdx.x * 8;
-    float held[kHeld][8], most = 0.0f;
+    // the largest of a chunk, by the 16 threads that have it
+    auto largest = [](const float (&v)[8]) {
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        return most;
+    };
+    // loops run over the vectors of whole warps, whose lanes stay together
+    const int step = blockDim.x * 8, lane = threadIdx.x & 31, lead = lane * 8, first = threadIdx.x * 8 - lead;
+    float held[kHeld][8], most = 0.0f, least = FLT_MAX;  // the largest of the row, and the smallest chunk's that is not 0
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        const int c = first + i * step;
+        const int c = first + lead + i * step;
 #pragma unroll
         for (int j = 0; j < 8; ++j) held[i][j] = 0.0f;
         if (c < k) load(c, held[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(held[i][j]));
+        const float m = largest(held[i]);
+        most = fmaxf(most, m);
+        if (m > 0.0f) least = fminf(least, m);
     }
-    for (int c = first + kHeld * step; c < k; c += step) {
-        float v[8];
-        load(c, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+    for (int c0 = first + kHeld * step; c0 < k; c0 += step) {
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (c0 + lead < k) load(c0 + lead, v);
+        const float m = largest(v);
+        most = fmaxf(most, m);
+        if (m > 0.0f) least = fminf(least, m);
     }
-    most = warp_max_nonneg(most);
-    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 16));
+    if (lane == 0) {
+        s_most[threadIdx.x >> 5] = most;
+        s_least[threadIdx.x >> 5] = least;
+    }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) most = fmaxf(most, s_most[w]);
-    const float scale = pow2_scale_for(most), inv = pow2_recip(scale);
-    if (threadIdx.x == 0) facts[r] = scale;
-    auto store = [&](int c, const float (&x8)[8]) {
+    for (int w = 0; w < 8; ++w) {
+        most = fmaxf(most, s_most[w]);
+        least = fminf(least, s_least[w]);
+    }
+    const int row_exp = terms_exp(most);
+    const bool own = most > 0.0f && row_exp - terms_exp(least) > kNear;
+    auto store = [&](int c, const float (&x8)[8], float m) {
+        int e = row_exp;
+        if (own && m > 0.0f) {
+            const int near = terms_exp(m);
+            if (row_exp - near > kNear) e = near;
+        }
+        const float scale = __uint_as_float(uint32_t(e) << 23), inv = pow2_recip(scale);
+        if (c % kChunk == 0) facts[int64_t(c / kChunk) * rows + r] = own ? -scale : scale;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x8[j] * inv;
@@ -204,12 +243,16 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
         }
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        if (first + i * step < width) store(first + i * step, held[i]);
-    for (int c = first + kHeld * step; c < width; c += step) {
+    for (int i = 0; i < kHeld; ++i) {
+        const int c = first + lead + i * step;
+        const float m = own ? largest(held[i]) : 0.0f;
+        if (c < width) store(c, held[i], m);
+    }
+    for (int c0 = first + kHeld * step; c0 < width; c0 += step) {
         float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (c < k) load(c, v);
-        store(c, v);
+        if (c0 + lead < k) load(c0 + lead, v);
+        const float m = own ? largest(v) : 0.0f;
+        if (c0 + lead < width) store(c0 + lead, v, m);
     }
 }
 
@@ -255,7 +298,7 @@ __host__ __device__ constexpr int acc_columns(int terms, int tile) {
 struct Int4Args {
     Geom g;
     const uint8_t* data;
-    const float* facts;      // the rows' scales; e4m3: [chunks][R] of x's, kFactBytes each
+    const float* facts;      // of split_x_kernel
     const int32_t* offsets;  // null: every row belongs to expert 0
     int R;
     void* out;
@@ -390,6 +433,12 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
     return false;
 }
 
+// A copy of 4 bytes to shared memory, and the wait for all of this thread's.
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
+
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
@@ -506,6 +555,7 @@ struct Shared {
     uint64_t ready[kMaxBufs], done[kMaxBufs];
     uint64_t join[2];
     uint32_t tmem;
+    bool own[kSets * 4];
 };
 
 // The work of one CTA: its items, and its steps of k in each.
@@ -680,23 +730,46 @@ __device__ __forceinline__ void load_piece(uint32_t d, int half, uint32_t* v) {
 }
 
 // One item: the sums of ROWS rows of x over the steps of this set of output warps, for this thread's weight
-// row.
-template <int TERMS, int GROUPS, int ROWS>
-__device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, int row, uint32_t lanes,
-                                           Ring& s, Ring& b, int& turn, float (&acc)[ROWS]) {
+// row.  Without OWN a row's terms have one power of two, which its sums then lack; with it each chunk's is a factor.
+// `mine`: 8 times 32 floats of this warp alone, kRows apart, for these of a step's chunks and of the next step's, whose
+// copies are in flight meanwhile.
+template <int TERMS, int GROUPS, int ROWS, bool OWN>
+__device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const Span& sp, const Item& it, int row,
+                                           uint32_t lanes, float* mine, Ring& s, Ring& b, int& turn, float (&acc)[ROWS]) {
     // a row's columns; rows whose columns are in registers at a time
     constexpr int kAccs = TERMS == 1 ? 1 : 2, kCols = 16, kFit = kCols / kAccs;
     constexpr int kAt = ROWS < kFit ? ROWS : kFit, kGo = kAt == ROWS && kAt * kAccs < kCols ? kCols / (kAt * kAccs) : 1;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) acc[t] = 0.0f;
+    int half = 0;  // of `mine`
+    auto fetch = [&](int c) {  // lane t: of row t
+        if (lane < it.rows && c < sp.step1) {
+            const float* fact = a.facts + int64_t(c) * a.step * a.R + it.row + lane;
+            const int n = min(a.step, a.g.chunks - c * a.step);
+#pragma unroll
+            for (int h = 0; h < kMaxStep; ++h)
+                if (h < n) cp_async4(mine + (half + h) * kRows + lane, fact + int64_t(h) * a.R);
+        }
+    };
+    if constexpr (OWN) fetch(sp.step0 + turn);
     for (int c = sp.step0; c < sp.step1; ++c, s.next(a.stages), b.next(a.bufs)) {
         if (turn != 0) {
             --turn;
             continue;
         }
         turn = kSets - 1;
-        if (!warp_wait(&sh.done[b.i], b.phase, a.err)) return false;
+        const float* facts = mine + half * kRows;
+        if constexpr (OWN) {
+            cp_async_wait();
+            __syncwarp();
+            half ^= kMaxStep;
+            fetch(c + kSets);
+        }
+        if (!warp_wait(&sh.done[b.i], b.phase, a.err)) {
+            if constexpr (OWN) cp_async_wait();
+            return false;
+        }
         tc_fence_after();
         const uint8_t* stage = s_ring + s.i * a.stage_bytes;
         const int n = min(a.step, a.g.chunks - c * a.step) * GROUPS;  // accumulators of the step
@@ -724,9 +797,14 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
 #pragma unroll
                 for (int k = 0; k < kGo; ++k) {
                     if (k > 0 && p + k >= n) break;
+                    float4 f;
 #pragma unroll
                     for (int t = 0; t < kAt; ++t) {
-                        float y;
+                        float y, w = scale[k];
+                        if constexpr (OWN) {
+                            if (t % 4 == 0) f = *reinterpret_cast<const float4*>(facts + (p + k) / GROUPS * kRows + t0 + t);
+                            w *= t % 4 == 0 ? f.x : t % 4 == 1 ? f.y : t % 4 == 2 ? f.z : f.w;
+                        }
                         if constexpr (TERMS == 1) y = __uint_as_float(v[k][t]);
                         if constexpr (TERMS == 2)
                             y = fmaf(__uint_as_float(v[k][2 * t + 1]), 0.0625f, __uint_as_float(v[k][2 * t]));
@@ -734,7 +812,7 @@ __device__ __forceinline__ bool accumulate(const Int4Args& a, Shared& sh, const 
                             y = fmaf(__uint_as_float(v[k][kAt + t]), 1.0f / 512, __uint_as_float(v[k][t]));
                         if constexpr (TERMS == 1)
                             y *= *reinterpret_cast<const float*>(stage + a.f_at + ((p + k) / GROUPS * a.tile + t0 + t) * kFactBytes);
-                        acc[t0 + t] = fmaf(y, scale[k], acc[t0 + t]);
+                        acc[t0 + t] = fmaf(y, w, acc[t0 + t]);
                     }
                 }
             }
@@ -764,7 +842,24 @@ __device__ __forceinline__ void write_out(const Int4Args& a, const Item& it, int
 
 __device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kSets * 128) : "memory"); }
 
-template <int TERMS, int GROUPS>
+// Whether any row has a chunk with a power of two of its own: the output warps' look at all rows of experts, while the
+// first products are under way.
+__device__ __forceinline__ bool any_own(const Int4Args& a, Shared& sh) {
+    const int warp = (int(threadIdx.x) >> 5) - kWarpOut;
+    bool own = false;
+#pragma unroll 4
+    for (int r = sh.row[0] + int(threadIdx.x) - kWarpOut * 32; r < sh.row[a.g.E]; r += kSets * 128)
+        own |= __ldcg(a.facts + r) < 0.0f;
+    own = __any_sync(0xffffffffu, own);
+    if ((threadIdx.x & 31) == 0) sh.own[warp] = own;
+    output_sync();
+    own = false;
+#pragma unroll
+    for (int w = 0; w < kSets * 4; ++w) own |= sh.own[w];
+    return own;
+}
+
+template <int TERMS, int GROUPS, bool OWN>
 __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s_part, const Span& sp, int rank) {
     const int lane = threadIdx.x & 31, quarter = (int(threadIdx.x) >> 5) & 3, row = quarter * 32 + lane;
     const int set = ((int(threadIdx.x) >> 5) - kWarpOut) >> 2, size = a.tile * kRows;
@@ -773,26 +868,23 @@ __device__ __forceinline__ void out_role(const Int4Args& a, Shared& sh, float* s
     Ring s, b;
     bool alive = true;
     uint32_t turn = 0;
-    if (lane == 0 && set == 0)  // no accumulators to take before the first products
-        for (int j = 0; j < a.bufs; ++j) mbar_arrive(&sh.ready[j]);
-    // The rows' scales are split_x_kernel's.  A CTA whose cluster has more CTAs than its items have steps of k waits for
-    // no product before it reads them.
-    if constexpr (TERMS > 1) chain_wait();
     for (int64_t i = sp.first; i < sp.items; i += sp.step, ++turn) {
         const Item it = find_item(a, sh.tile, sh.row, i);
         float* part = s_part + (a.ranks > 1 ? (turn & 1) * kSets * size : 0);  // [set][row of x][weight row]
         auto item = [&](auto rows) {
             constexpr int ROWS = decltype(rows)::value;
             float acc[ROWS];
-            alive = alive && accumulate<TERMS, GROUPS, ROWS>(a, sh, sp, row, lanes, s, b, wait_turns, acc);
+            alive = alive && accumulate<TERMS, GROUPS, ROWS, OWN>(a, sh, sp, it, row, lanes, part + set * size + quarter * 32, s,
+                                                                   b, wait_turns, acc);
 #pragma unroll
             for (int t = 0; t < ROWS; ++t) part[set * size + t * kRows + row] = acc[t];
         };
         if (it.rows <= 8) item(std::integral_constant<int, 8>{});
         else if (it.rows <= 16) item(std::integral_constant<int, 16>{});
         else item(std::integral_constant<int, 32>{});
-        // Lane t has the scale of row t.
-        const float scale = TERMS > 1 && lane < it.rows ? __ldcg(a.facts + it.row + lane) : 1.0f;
+        // Lane t has what the sums of row t lack.
+        float scale = TERMS > 1 && lane < it.rows ? __ldcg(a.facts + it.row + lane) : 1.0f;
+        if constexpr (OWN) scale = scale < 0.0f ? -1.0f : 1.0f;
         int t0 = 0, t1 = it.rows;
         output_sync();
         if (a.ranks > 1) {
@@ -886,6 +978,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
     } else if (warp < kWarpOut) {
         widen_role<GROUPS>(a, sh, sp);
     } else {
+        if ((threadIdx.x & 31) == 0 && warp < kWarpOut + 4)  // no accumulators to take before the first products
+            for (int j = 0; j < a.bufs; ++j) mbar_arrive(&sh.ready[j]);
         // rows of no expert
         const int used = sh.row[g.E], lead = sh.row[0];
         const int64_t outside = int64_t(lead) + (a.R - used);
@@ -893,7 +987,13 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
             for (int n = int(threadIdx.x) - kWarpOut * 32; n < g.out_n; n += kSets * 128)
                 store1(a.out, a.out_dtype, (r < lead ? r : r - lead + used) * a.ld_out + n, 0.0f);
         }
-        out_role<TERMS, GROUPS>(a, sh, s_part, sp, rank);
+        if constexpr (TERMS > 1) {
+            chain_wait();  // the facts are split_x_kernel's
+            if (any_own(a, sh)) out_role<TERMS, GROUPS, true>(a, sh, s_part, sp, rank);
+            else out_role<TERMS, GROUPS, false>(a, sh, s_part, sp, rank);
+        } else {
+            out_role<TERMS, GROUPS, false>(a, sh, s_part, sp, rank);
+        }
     }
     __syncwarp();
     tc_fence_before();
@@ -1127,7 +1227,7 @@ extern "C" int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int
     if (R < 0 || !bytes) return set_last_error(CST_ERR_INVALID_ARG, "R=%d must be >= 0 and bytes not null", R);
     const Geom g = make_geom(*w);
     const int terms = terms_of(x_dtype);
-    *bytes = terms_bytes(g, terms, R) + int64_t(R) * (terms == 1 ? g.chunks * kFactBytes : 4);
+    *bytes = terms_bytes(g, terms, R) + int64_t(R) * g.chunks * (terms == 1 ? kFactBytes : 4);
     return CST_OK;
 }
 

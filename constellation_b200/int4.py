@@ -137,9 +137,10 @@ def grouped_int4(x: torch.Tensor, w: Int4Weight, offsets: torch.Tensor | None = 
     ``[R, N]`` (``[R, N / 2]`` with swiglu) in ``out_dtype``: fp16, bf16 or fp32; by default ``x``'s type, bf16
     for e4m3 rows.  ``out`` may not overlap ``x``, ``x_scale``, ``offsets`` or the weight's ``data``.
 
-    fp32 sums, one rounding.  fp16 and bf16 rows enter as 8-bit terms: exactly where a number is above 2^-11 (fp16)
-    or 2^-13 (bf16) of its row's largest, and with an error below 2^-22 (2^-21) of that largest elsewhere.  So a row
-    whose outlier is 2^20 times the rest keeps little of the rest.  An infinity makes its row's results NaN."""
+    fp32 sums, one rounding.  fp16 and bf16 rows enter as 8-bit terms: exactly where a number is above 2^-11 (fp16) or
+    2^-13 (bf16) of its row's largest, and with an error below 2^-22 (2^-21) of that largest elsewhere, which is also
+    below 2^-18 (2^-17) of the largest of its 128 columns.  Rows whose 128-column blocks differ by 5 binades or more, as
+    around outliers, take up to 1.35 times as long.  An infinity makes its row's results NaN."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda:
         raise TypeError("grouped_int4 expects a 2-D CUDA tensor")
     dev = x.device

@@ -333,7 +333,8 @@ int cst_int4_workspace(const cst_int4_weight* w, int32_t x_dtype, int32_t R, int
  * `out` may not overlap x, x_scale, offsets, data or workspace, which are read while it is written
  * (CST_ERR_INVALID_ARG); it may be other columns of x's array, at the same row pitch in bytes.
  * x enters the products as 8-bit terms that hold it exactly but for what is below 2^-21 (bf16) or
- * 2^-22 (fp16) of the largest |x| of its row; sums are fp32, with one rounding.
+ * 2^-22 (fp16) of the largest |x| of its row, and below 2^-17 (2^-18) of that of its 128 columns;
+ * sums are fp32, with one rounding.
  * An infinity in a row of x makes the row's results NaN.  `data` is only read, but for its error word. */
 int cst_grouped_int4(const cst_int4_weight* w, void* data, const void* x, int32_t x_dtype, int64_t ld_x,
                      const float* x_scale, int64_t ld_x_scale, const int32_t* offsets, int32_t R, void* workspace,

@@ -144,3 +144,110 @@ def test_out_beside_the_inputs():
                                          room.data_ptr(), wide.data_ptr() + 512, 2, 320,
                                          torch.cuda.current_stream().cuda_stream))
     assert torch.equal(wide[:, 256:], grouped_int4(xb, w, off)) and torch.equal(wide[:, :256], xb)
+
+
+def check_chunks(out, x, W, group, dt):
+    """Against W x in 64 bits: the sums' rounding, and what terms may drop of a number, which goes by the largest of its
+    128 columns.  Terms fit the largest of a row to 448 and drop at most 2^-14 of their power of two (bf16: half of
+    e4m3's smallest step of 2^-9, over 16; fp16: the third term is 512 times a rest below 2^-10, and rounded to half a
+    step of 2^-5: 2^-15).  A chunk takes its own where its largest is 5 binades below, so its power of two is at most
+    2^4 times the smallest that fits its largest, which is above 224 of that: 2^-14 * 2^4 / 224 < 2^-17."""
+    K, x64 = W.shape[1], x.double()
+    most = torch.stack([c.abs().amax(1) for c in x64.split(128, 1)], 1)
+    sizes = torch.stack([c.abs().sum(1) for c in W.split(128, 1)], 1)
+    ref = x64 @ W.T
+    err = (group + 2 * K / group + 64) * 2.0 ** -23 * (x64.abs() @ W.abs().T) + 2.0 ** -17 * (most @ sizes.T)
+    bound = err + ref.abs() * 2.0 ** -24 + 2.0 ** -126
+    got = out.double()
+    assert ((got - ref).abs() <= bound).all(), ((got - ref).abs() / bound).max()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,N,K,group,zeros", [(1, 136, 640, 128, False), (8, 2048, 2560, 128, False),
+                                               (13, 200, 1152, 64, True), (40, 144, 2048, 128, True),
+                                               (70, 96, 864, 32, False), (5, 64, 10240, 128, False),
+                                               (600, 1024, 1024, 128, False)])
+def test_an_outlier_costs_the_others_nothing(R, N, K, group, zeros, dt):
+    """Numbers 10^4.8 times the rest in a group of weights that is all zero: what is left are the other columns, and they
+    have as many bits as if the outlier were not there."""
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    q, s, z, W = make_weight(1, N, K, group, zeros)
+    at = K // 2 // 128 * 128  # a chunk's first column, and the groups of that chunk
+    s[:, :, at // group:(at + 128) // group] = 0
+    W[:, :, at:at + 128] = 0
+    w = Int4Weight(q, s, z)
+    x, _, _ = make_x(R, K, torch.float32)
+    plain = x.to(dt)
+    x[:, at + 3] = 60000.0
+    x[::3, at + 40] = -3000.0
+    if R > 2:
+        x[1, at + 3] = 0.5  # a row without one
+        x[2] *= 2.0 ** -6
+        x[2, 128:] *= 2.0 ** -7  # and one whose chunks differ
+        plain[1:3] = x[1:3].to(dt)
+    x = x.to(dt)
+    out = grouped_int4(x, w, out_dtype=torch.float32)
+    check_chunks(out, x, W[0], group, dt)
+    assert torch.equal(grouped_int4(x, w, out_dtype=torch.float32), out)
+    if R > 2:  # rows do not depend on the rows beside them
+        plain[0] = plain[1]
+        plain[2] = plain[1]
+        assert torch.equal(grouped_int4(plain, w, out_dtype=torch.float32)[1], out[1])
+
+
+@gpu
+@pytest.mark.parametrize("factor", [2.0 ** 30, 2.0 ** 90, 2.0 ** 120])
+def test_chunks_of_every_size_in_a_row(factor):
+    """bf16 chunks far apart, beside chunks of zeros: each keeps its bits where the larger ones' weights are zero."""
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    N, K, R = 96, 1024, 11
+    q, s, z, W = make_weight(1, N, K, 128, False, torch.float32)
+    x, _, _ = make_x(R, K, torch.float32)
+    x[:, 256:384] *= factor
+    x[:, 512:640] /= factor
+    x[::2, 768:896] = 0
+    x = x.to(torch.bfloat16)
+    for held in ([0, 1, 3, 4, 5, 6, 7], [4], [2], [2, 4, 6]):
+        keep = torch.zeros(K // 128, dtype=torch.bool)
+        keep[held] = True
+        s1 = torch.where(keep.cuda(), s, torch.zeros((), device="cuda"))
+        W1 = W * keep.cuda().double().repeat_interleave(128)
+        out = grouped_int4(x, Int4Weight(q, s1, z), out_dtype=torch.float32)
+        assert torch.isfinite(out).all()
+        check_chunks(out, x, W1[0], 128, torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_outliers_among_experts(dt):
+    """Experts of one and of many rows with and without outliers, NaN in a row, and rows of no expert full of both."""
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    counts, N, K = (3, 0, 40, 9, 1, 17), 160, 1280
+    q, s, z, W = make_weight(len(counts), N, K, 128, True)
+    w, off, R = Int4Weight(q, s, z), offsets_of(counts), sum(counts)
+    x, _, _ = make_x(R + 4, K, torch.float32)
+    x[::5, 700] = 9000.0
+    x[R:] = 1e-6
+    x[R:, 5] = 60000.0
+    x = x.to(dt)
+    clean = grouped_int4(x, w, off, out_dtype=torch.float32)
+    assert (clean[R:] == 0).all()
+    for e, (lo, hi) in enumerate(zip(off.tolist(), off.tolist()[1:])):
+        if hi > lo:
+            # zero points take part in the sums, so that their magnitude is that of scale (q + zero) |x|
+            most = x[lo:hi].double().abs()
+            v = torch.stack((q[e] & 15, q[e] >> 4), -1).view(N, K).double() + z[e].double().repeat_interleave(128, 1)
+            mag = v * s[e].double().repeat_interleave(128, 1)
+            ref = x[lo:hi].double() @ W[e].T
+            bound = (128 + 2 * K / 128 + 64) * 2.0 ** -23 * (most @ mag.T) + 2.0 ** -17 * (
+                torch.stack([c.amax(1) for c in most.split(128, 1)], 1)
+                @ torch.stack([c.abs().sum(1) for c in W[e].split(128, 1)], 1).T) + ref.abs() * 2.0 ** -24
+            assert ((clean[lo:hi].double() - ref).abs() <= bound).all()
+    x[7, 3], x[48, 1279] = float("nan"), float("inf")
+    out = grouped_int4(x, w, off, out_dtype=torch.float32)
+    keep = [r for r in range(R) if r not in (7, 48)]
+    assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[[7, 48]]).any()
