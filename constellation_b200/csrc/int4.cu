@@ -126,8 +126,8 @@ __device__ __forceinline__ int terms_exp(float most) { return int(__float_as_uin
 // One CTA a row.  terms: [rows * TERMS][chunks * 128] (of three terms [t1, t3, t2][rows][chunks * 128], so that one
 // product takes t1 and t3), columns past k zero.  facts: [chunks][rows] of the power of two of a row's terms in a
 // chunk, negative in all of a row that has a chunk with one of its own; for e4m3 (TERMS 1) of x_scale, 16 bytes each.
-// A chunk is 8 columns of 16 threads, who find its largest by shuffles.  A row's first 8192 columns stay in registers
-// between its maximum and its terms; more are read twice.
+// A chunk is 8 columns of 16 threads, who find its largest by shuffles.  A row's first 8192 columns (256 threads) stay in
+// registers between its maximum and its terms; more are read twice.
 template <int TERMS>
 __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype, int64_t ld, const float* x_scale,
                                                       int64_t ld_xs, int rows, int k, uint8_t* terms, float* facts) {
@@ -171,37 +171,36 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
         for (int j = 0; j < 8; ++j)
             if (isinf(v[j])) v[j] = __int_as_float(0x7fffffff);
     };
-    // the largest of a chunk, by the 16 threads that have it
-    auto largest = [](const float (&v)[8]) {
-        float most = 0.0f;
+    const int step = blockDim.x * 8, lane = threadIdx.x & 31, lead = lane * 8, first = threadIdx.x * 8 - lead;
+    // the largest of each of the two chunks that a warp has; a NaN is none
+    auto largest = [&](const float (&v)[8]) {
+        float m = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        return most;
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+        const uint32_t bits = __float_as_uint(m);  // in the order of the numbers, which are not negative
+        return make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, lane < 16 ? bits : 0u)),
+                           __uint_as_float(__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : bits)));
+    };
+    float held[kHeld][8], most = 0.0f, least = FLT_MAX;  // the largest of the row, and the smallest chunk's that is not 0
+    auto add = [&](float2 m) {
+        most = fmaxf(most, fmaxf(m.x, m.y));
+        least = fminf(least, fminf(m.x > 0.0f ? m.x : FLT_MAX, m.y > 0.0f ? m.y : FLT_MAX));
     };
     // loops run over the vectors of whole warps, whose lanes stay together
-    const int step = blockDim.x * 8, lane = threadIdx.x & 31, lead = lane * 8, first = threadIdx.x * 8 - lead;
-    float held[kHeld][8], most = 0.0f, least = FLT_MAX;  // the largest of the row, and the smallest chunk's that is not 0
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        const int c = first + lead + i * step;
 #pragma unroll
         for (int j = 0; j < 8; ++j) held[i][j] = 0.0f;
-        if (c < k) load(c, held[i]);
-        const float m = largest(held[i]);
-        most = fmaxf(most, m);
-        if (m > 0.0f) least = fminf(least, m);
+        if (first + lead + i * step < k) load(first + lead + i * step, held[i]);
     }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (first + i * step < k) add(largest(held[i]));
     for (int c0 = first + kHeld * step; c0 < k; c0 += step) {
         float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (c0 + lead < k) load(c0 + lead, v);
-        const float m = largest(v);
-        most = fmaxf(most, m);
-        if (m > 0.0f) least = fminf(least, m);
+        add(largest(v));
     }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 16));
     if (lane == 0) {
         s_most[threadIdx.x >> 5] = most;
         s_least[threadIdx.x >> 5] = least;
@@ -209,12 +208,14 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
+        if (w >= int(blockDim.x >> 5)) break;
         most = fmaxf(most, s_most[w]);
         least = fminf(least, s_least[w]);
     }
     const int row_exp = terms_exp(most);
     const bool own = most > 0.0f && row_exp - terms_exp(least) > kNear;
-    auto store = [&](int c, const float (&x8)[8], float m) {
+    auto store = [&](int c, const float (&x8)[8], float2 both) {
+        const float m = lane < 16 ? both.x : both.y;
         int e = row_exp;
         if (own && m > 0.0f) {
             const int near = terms_exp(m);
@@ -245,13 +246,14 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int c = first + lead + i * step;
-        const float m = own ? largest(held[i]) : 0.0f;
+        if (c - lead >= width) continue;
+        const float2 m = own ? largest(held[i]) : make_float2(0.0f, 0.0f);
         if (c < width) store(c, held[i], m);
     }
     for (int c0 = first + kHeld * step; c0 < width; c0 += step) {
         float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (c0 + lead < k) load(c0 + lead, v);
-        const float m = own ? largest(v) : 0.0f;
+        const float2 m = own ? largest(v) : make_float2(0.0f, 0.0f);
         if (c0 + lead < width) store(c0 + lead, v, m);
     }
 }
@@ -842,14 +844,26 @@ __device__ __forceinline__ void write_out(const Int4Args& a, const Item& it, int
 
 __device__ __forceinline__ void output_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(kSets * 128) : "memory"); }
 
-// Whether any row has a chunk with a power of two of its own: the output warps' look at all rows of experts, while the
-// first products are under way.
-__device__ __forceinline__ bool any_own(const Int4Args& a, Shared& sh) {
-    const int warp = (int(threadIdx.x) >> 5) - kWarpOut;
+// Whether a row has a chunk with a power of two of its own: the output warps' look at the rows while the first products are
+// under way.  At all rows of experts, while that is one wait for memory; of more, each thread looks at an item's of this
+// CTA's (131072 bf16 rows over 64 experts [256, 128]: 396 us, and 123 us more with a look at all rows).
+__device__ __forceinline__ bool any_own(const Int4Args& a, Shared& sh, const Span& sp) {
+    const int me = int(threadIdx.x) - kWarpOut * 32, warp = me >> 5, first = sh.row[0], last = sh.row[a.g.E];
+    constexpr int kAtOnce = 8;
     bool own = false;
-#pragma unroll 4
-    for (int r = sh.row[0] + int(threadIdx.x) - kWarpOut * 32; r < sh.row[a.g.E]; r += kSets * 128)
-        own |= __ldcg(a.facts + r) < 0.0f;
+    if (last - first <= kAtOnce * kSets * 128) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int r = first + me + i * kSets * 128;
+            if (r < last) own |= __ldcg(a.facts + r) < 0.0f;
+        }
+    } else {
+        for (int64_t i = sp.first + me * sp.step; i < sp.items; i += kSets * 128 * sp.step) {
+            const Item it = find_item(a, sh.tile, sh.row, i);
+#pragma unroll 8
+            for (int t = 0; t < it.rows; ++t) own |= __ldcg(a.facts + it.row + t) < 0.0f;
+        }
+    }
     own = __any_sync(0xffffffffu, own);
     if ((threadIdx.x & 31) == 0) sh.own[warp] = own;
     output_sync();
@@ -989,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_kernel(const __grid_constant
         }
         if constexpr (TERMS > 1) {
             chain_wait();  // the facts are split_x_kernel's
-            if (any_own(a, sh)) out_role<TERMS, GROUPS, true>(a, sh, s_part, sp, rank);
+            if (any_own(a, sh, sp)) out_role<TERMS, GROUPS, true>(a, sh, s_part, sp, rank);
             else out_role<TERMS, GROUPS, false>(a, sh, s_part, sp, rank);
         } else {
             out_role<TERMS, GROUPS, false>(a, sh, s_part, sp, rank);
@@ -1120,7 +1134,9 @@ int launch_terms(Int4Args a, const void* x, int x_dtype, int64_t ld_x, const flo
                  void* workspace, int sms, cudaStream_t s) {
     float* facts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + terms_bytes(a.g, TERMS, a.R));
     a.facts = facts;
-    const cudaError_t e = launch_chained(split_x_kernel<TERMS>, dim3(unsigned(a.R)), dim3(256), 0, s, x, x_dtype, ld_x,
+    // a thread for 8 columns, up to 256 (131072 rows of k = 128: 138 us, with 256 threads 364)
+    const int threads = a.g.chunks >= 16 ? 256 : (a.g.chunks + 1) / 2 * 32;
+    const cudaError_t e = launch_chained(split_x_kernel<TERMS>, dim3(unsigned(a.R)), dim3(threads), 0, s, x, x_dtype, ld_x,
                                          x_scale, ld_xs, a.R, a.g.K, static_cast<uint8_t*>(workspace), facts);
     if (e != cudaSuccess) return set_last_error(CST_ERR_CUDA, "split_x launch failed: %s", cudaGetErrorString(e));
     return a.g.group == 128  ? launch_int4<TERMS, 1>(a, workspace, sms, s)
