@@ -251,3 +251,56 @@ def test_outliers_among_experts(dt):
     out = grouped_int4(x, w, off, out_dtype=torch.float32)
     keep = [r for r in range(R) if r not in (7, 48)]
     assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[[7, 48]]).any()
+
+
+@gpu
+@pytest.mark.parametrize("outlier", [False, True])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_items_one_after_the_other_in_a_cluster(dt, outlier):
+    """160 items of 21 steps over pairs of CTAs: a pair's sums of one item lie beside those of the next."""
+    from constellation_b200.int4 import Int4Weight
+
+    R, N, K = 40, 10240, 5376
+    q, s, z, W = make_weight(1, N, K, 128, False)
+    s[:, :, 20] = 0
+    W[:, :, 2560:2688] = 0
+    w = Int4Weight(q, s, z)
+    x = rows_of_every_size(R, K, dt)
+    if outlier:
+        x[:, 2600] = x.abs().amax(1) * (40.0 if dt == torch.float16 else 2.0 ** 17)
+    room = torch.full((w._workspace(1 if dt == torch.float16 else 2, R),), 0xFF, dtype=torch.uint8, device="cuda")
+    out = product_in(room, x, w, None)
+    check_chunks(out, x, W[0], 128, dt)
+    for _ in range(3):
+        assert torch.equal(product_in(room, x, w, None), out)
+
+
+@gpu
+def test_outliers_that_come_and_go_between_replays():
+    """Captured calls in two graphs on two streams at once, whose rows change between replays, and eager calls beside."""
+    from constellation_b200.int4 import Int4Weight, grouped_int4
+
+    q, s, z, W = make_weight(4, 512, 2048, 128, True)
+    w, off = Int4Weight(q, s, z), offsets_of((5, 0, 20, 2))
+    plain, _, _ = make_x(30, 2048, torch.bfloat16)
+    spiky = plain.clone()
+    spiky[::4, 77] = 2.0 ** 16
+    want = [grouped_int4(x, w, off, out_dtype=torch.float32) for x in (plain, spiky)]
+    xs, graphs, outs = [plain.clone(), spiky.clone()], [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(grouped_int4(x, w, off, out_dtype=torch.float32))
+    streams = [torch.cuda.Stream() for _ in xs]
+    for turn in range(6):
+        for i, x in enumerate(xs):
+            x.copy_((plain, spiky)[(i + turn) % 2])
+        torch.cuda.synchronize()
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                graphs[i].replay()
+        beside = grouped_int4(spiky, w, off, out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        assert torch.equal(beside, want[1])
+        assert all(torch.equal(outs[i], want[(i + turn) % 2]) for i in range(2)), turn
+    w.device_error()
