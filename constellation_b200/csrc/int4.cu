@@ -275,8 +275,8 @@ __global__ void __launch_bounds__(256) split_x_kernel(const void* x, int x_dtype
 // Bound: HBM up to about 8 rows an expert; above, the handing of steps from role to role (a step is 600 to 1500
 // cycles, in which no role is busy throughout), which is why a step holds as many chunks as tensor memory has
 // room for twice, and the widening (a third of the issue slots).  Up and gate [4096, 7168], groups of 128, bf16
-// rows: 32 experts of 1 row 84 us (5.7 TB/s of weights and rows), 64 experts of 8 rows 201 us (4.9 TB/s),
-// 32 experts of 32 rows 152 us (395 TFLOP/s).  Down [7168, 2048], groups of 64 with zero points, 254 fp16 rows over
+// rows: 32 experts of 1 row 91 us (5.3 TB/s of weights and rows), 64 experts of 8 rows 189 us (5.2 TB/s),
+// 32 experts of 32 rows 162 us (371 TFLOP/s).  Down [7168, 2048], groups of 64 with zero points, 254 fp16 rows over
 // 32 experts: 96 us (2.7 TB/s).  200 e4m3 rows over 8 experts of [4096, 7168]: 64 us, two and a third rounds
 // of items over the SMs taking three.
 // Operands of x's own 16-bit type instead of e4m3 terms would need no terms, but 9 to 11 operations for 8
