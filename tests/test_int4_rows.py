@@ -127,11 +127,11 @@ def test_out_beside_the_inputs():
         return buf[at:at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
 
     # x 2048 bytes, its scales 64, offsets 12, out 1024
-    x1, xs1, off1 = put(1024, x), put(3072, xs), put(3136, off)
-    for at in (0, 3152):
+    x1, xs1, off1 = put(1024, x), put(3200, xs), put(3264, off)
+    for at in (0, 3280):
         out = buf[at:at + 1024].view(torch.bfloat16).view(8, 64)
         assert torch.equal(grouped_int4(x1, w, off1, x_scale=xs1, out=out), want)
-    for at in (16, 1024, 2048, 3056, 3120, 3136):
+    for at in (16, 1024, 2048, 3184, 3248, 3264):
         out = buf[at:at + 1024].view(torch.bfloat16).view(8, 64)
         with pytest.raises(RuntimeError, match="overlaps"):
             grouped_int4(x1, w, off1, x_scale=xs1, out=out)
